@@ -149,6 +149,57 @@ int gpuq_schur_weights_dev(const double *d_u, int64_t ne0, float *d_w, int64_t n
 size_t gpuq_ldlq(int type, const float *W, const double *H, int64_t h_stride, double n, double damp, int order,
                  int weights, const float *imatrix, int64_t nmat, int64_t ne1, int64_t ne0, void *dst);
 
+/* ---- expert layers: MXFP4 rounding, products with stored MXFP4 matrices, routing (no counterpart in the reference,
+ * whose calibration pass runs inside llama.cpp or torch). All asynchronous on `stream`; capturable. ----
+ *
+ * A packed MXFP4 matrix [nrow][n_per_row] holds, with np = n_per_row rounded up to 512, the codes [nrow][np / 2] (value
+ * 2i in the low nibble of byte i) and then the scales [nrow][np / 32] (block 4c + q of each 16 at byte 4q + c); its
+ * padding is zero. gpuq_mxfp4_packed_bytes: its size, 0 for sizes that no call takes (n_per_row a multiple of 32, at most
+ * 2^24). A stack of nmat matrices is one packed matrix of nmat * ne1 rows. */
+size_t gpuq_mxfp4_packed_bytes(int64_t nrow, int64_t n_per_row);
+
+/* Rounds rows to MXFP4: d_src F32 / F16 / BF16 [nrow][n_per_row], ld elements from row to row (rows 16-byte aligned) ->
+ * d_dst, packed (1) or ggml's 17-byte blocks (0), and, where d_values is not NULL, the rounded values as BF16
+ * [nrow][n_per_row] (exact). A block of 32 shares 2^(floor(log2(largest)) - 2), its exponent clamped to what e8m0 holds;
+ * a value becomes the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (a tie the smaller, past 6 becomes 6, no negative
+ * zero). A NaN becomes 0, an infinity 6 * 2^125. src_type MXFP4 (ggml's blocks, ld = n_per_row) with packed 1 lays
+ * stored blocks out packed, bit for bit. d_dst, d_values and d_src (but MXFP4's) 16-byte aligned. Returns the bytes of
+ * d_dst, 0 on an error. */
+size_t gpuq_mxfp4_quantize_dev(int src_type, const void *d_src, int64_t nrow, int64_t n_per_row, int64_t ld, int packed,
+                               void *d_dst, void *d_values, void *stream);
+
+/* The scratch bytes gpuq_mxfp4_matmul_dev needs at d_work for nx rows of x_type (0 for BF16 and MXFP4: NULL will do) */
+size_t gpuq_mxfp4_matmul_work(int x_type, int64_t nx, int64_t ne0);
+
+/* Products of rows with packed MXFP4 matrices d_w [nmat][ne1][ne0]: y[r] = x[d_rows[r]] w[e]^T for the rows
+ * d_offsets[e] <= r < d_offsets[e + 1] of matrix e (int32, device; nmat 1: d_offsets may be NULL, all m rows). d_rows NULL:
+ * x[r]. With d_up (packed, the same sizes) SwiGLU: y = g / (1 + exp(-g)) * u, g of d_w and u of d_up. x_type: BF16, F16,
+ * F32 [nx][ld] (rows 16-byte aligned; no bit of x or w is rounded away, sums in f32) or packed MXFP4 (39, ld = ne0).
+ * y_type F32, F16 or BF16: d_y [m][ne1]. A row that no matrix has (r >= d_offsets[nmat]) or whose d_rows names no row of x
+ * is zero. A scale of 255 is NaN (unlike in ggml's to_float, which takes it for 2^128). At most 65534 matrices and 2^30
+ * rows; pointers 16-byte aligned (d_offsets, d_rows 4). Returns the bytes of d_y, 0 on an error. */
+size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx, int64_t ld, const void *d_w, const void *d_up,
+                             int64_t nmat, int64_t ne1, int64_t ne0, const int32_t *d_offsets, const int32_t *d_rows,
+                             int64_t m, int y_type, void *d_y, void *d_work, void *stream);
+
+/* A router's choice: the k best of nexp experts for each token of d_logits (F32 / F16 / BF16 [ntok][nexp], ld elements
+ * from row to row) -> d_ids [ntok][k] int32, best first, and d_weights [ntok][k] f32. score = softmax over all experts, or
+ * sigmoid; key = score + d_bias[e] (f32; NULL: none), or the logit itself with no bias and one group. ngroup groups of
+ * nexp / ngroup neighbours: a group counts by the sum of its two largest keys and the `keep` best groups stay. A tie goes
+ * to the lowest index. weight = scale * score, over the sum of the chosen scores with renorm (zero where that is zero).
+ * A NaN or minus infinity is never chosen; what is left over gets id -1 and weight 0. nexp <= 1024, k <= 64, ngroup <= 64.
+ * Returns 0; 1 bad arguments; 4 a HIP error. */
+int gpuq_route_dev(int type, const void *d_logits, int64_t ntok, int64_t ld, int nexp, int k, int sigmoid,
+                   const float *d_bias, int ngroup, int keep, int renorm, float scale, int32_t *d_ids, float *d_weights,
+                   void *stream);
+
+/* Sorts the assignments of d_ids [ntok][k] by expert, in order within each: d_offsets [nexp + 1], d_rows [ntok * k] the
+ * token of each place and d_slots [ntok * k] its index in d_ids. Ids that name no expert come last, as -1 in both.
+ * d_work: gpuq_route_group_work(ntok * k, nexp) bytes (NULL where that is 0). Returns 0; 1 bad arguments; 4 a HIP error. */
+size_t gpuq_route_group_work(int64_t n, int nexp);
+int gpuq_route_group_dev(const int32_t *d_ids, int64_t ntok, int k, int nexp, int32_t *d_offsets, int32_t *d_rows,
+                         int32_t *d_slots, void *d_work, void *stream);
+
 /* Reads and clears the flag the kernels set where the reference would trap (a key with no candidate point: non-
  * finite input or an inconsistent table). Synchronizes the device. */
 int gpuq_take_error(void);

@@ -705,6 +705,9 @@ bool launch_solve(int type, const float *W, const uint8_t *q, int64_t q_stride, 
 
 }  // namespace
 
+// for the library's other source files
+__attribute__((visibility("hidden"))) int gq_device(void) { return g_device; }
+
 // ------------------------------------------------------------------ the C ABI
 extern "C" int gpuq_init(const char *tables, int device) {
     std::lock_guard<std::mutex> lock(g_mu);

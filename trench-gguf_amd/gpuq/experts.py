@@ -1,0 +1,145 @@
+"""Expert layers on the device: a router's choice, rounding to MXFP4 and products with stored MXFP4 experts.
+
+A mixture-of-experts layer's calibration pass needs these around the quantizer: `route` chooses experts from the
+router's logits, `group` sorts the chosen rows by expert, `pack` lays a GGUF file's MXFP4 tensor out for products and
+`matmul` multiplies rows with it (a stack with its grouping in one call, gate and up with SwiGLU in one pass);
+`quantize` and `quantize_blocks` round rows to MXFP4 themselves. torch only holds the device memory; every call enqueues
+on torch's current stream and returns without synchronizing, and raises ValueError for arguments the library refuses.
+`gpuq/calibrate.py` runs them together.
+"""
+from collections import namedtuple
+
+import torch
+
+from gpuq import BF16, F16, F32, MXFP4
+
+TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+# a packed MXFP4 tensor on the device: the bytes and [nmat, ne1, ne0] (rows: nmat 1)
+Packed = namedtuple("Packed", "data nmat ne1 ne0")
+# assignments sorted by expert: offsets [nexp + 1], the token of each place and its index among the ids, all int32
+Group = namedtuple("Group", "offsets rows slots")
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _rows(x):
+    """(type, pointer, rows, columns, elements from row to row) of a 2-d float tensor whose rows are contiguous"""
+    if x.dim() != 2 or x.dtype not in TYPES or not x.is_cuda:
+        raise ValueError("expected a 2-d F32 / F16 / BF16 tensor on the GPU")
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        raise ValueError("rows must be contiguous")
+    ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    return TYPES[x.dtype], x.data_ptr(), x.shape[0], x.shape[1], ld
+
+
+def pack(gq, blocks, nmat, ne1, ne0):
+    """ggml's MXFP4 blocks (uint8 on the device, nmat x ne1 rows of ne0 values) -> Packed, bit for bit"""
+    if blocks.dtype != torch.uint8 or not blocks.is_contiguous() or ne0 % 32 or \
+            blocks.numel() != nmat * ne1 * (ne0 // 32) * 17:
+        raise ValueError("expected %d contiguous bytes of MXFP4 blocks" % (nmat * ne1 * (ne0 // 32) * 17))
+    size = gq.gpuq_mxfp4_packed_bytes(nmat * ne1, ne0)
+    out = torch.empty(size, dtype=torch.uint8, device=blocks.device)
+    if not size or gq.gpuq_mxfp4_quantize_dev(MXFP4, blocks.data_ptr(), nmat * ne1, ne0, ne0, 1, out.data_ptr(), None,
+                                              _stream(blocks)) != size:
+        raise ValueError("gpuq_mxfp4_quantize_dev refused %d x %d x %d blocks" % (nmat, ne1, ne0))
+    return Packed(out, nmat, ne1, ne0)
+
+
+def _quantize(gq, x, packed, values):
+    typ, ptr, n, ncol, ld = _rows(x)
+    size = gq.gpuq_mxfp4_packed_bytes(n, ncol) if packed else n * (ncol // 32) * 17
+    out = torch.empty(size, dtype=torch.uint8, device=x.device)
+    back = torch.empty((n, ncol), dtype=torch.bfloat16, device=x.device) if values else None
+    got = gq.gpuq_mxfp4_quantize_dev(typ, ptr, n, ncol, ld, int(packed), out.data_ptr(),
+                                     back.data_ptr() if values else None, _stream(x)) if size else 0
+    if not got or got != size:
+        raise ValueError("gpuq_mxfp4_quantize_dev refused %d x %d (rows of whole 32s, 16-byte aligned)" % (n, ncol))
+    return out, back
+
+
+def quantize(gq, x, values=False):
+    """rows rounded to MXFP4, Packed; with values also what they stand for, BF16 [n, ncol]: (Packed, values)"""
+    out, back = _quantize(gq, x, True, values)
+    p = Packed(out, 1, x.shape[0], x.shape[1])
+    return (p, back) if values else p
+
+
+def quantize_blocks(gq, x, values=False):
+    """rows rounded to MXFP4 as ggml's blocks, uint8 [n, ncol / 32 * 17]; with values (blocks, values)"""
+    out, back = _quantize(gq, x, False, values)
+    out = out.view(x.shape[0], -1)
+    return (out, back) if values else out
+
+
+def _index(t, name):
+    if t.dtype != torch.int32 or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError("%s must be contiguous int32 on the GPU" % name)
+    return t.data_ptr()
+
+
+def matmul(gq, x, w, group=None, up=None, out_dtype=torch.float32):
+    """x [n, ne0] (F32, F16, BF16 or Packed rows) times w (Packed [nmat, ne1, ne0]) transposed -> [m, ne1].
+
+    Without a group m = n and w is one matrix; with one (Group, from `group`) output row r is x[group.rows[r]] times the
+    matrix whose offsets hold r, zero where none does. up: a second Packed like w, for silu(x w^T) * (x up^T)."""
+    if isinstance(x, Packed):
+        typ, ptr, n, ncol, ld, dev = MXFP4, x.data.data_ptr(), x.nmat * x.ne1, x.ne0, x.ne0, x.data.device
+    else:
+        typ, ptr, n, ncol, ld = _rows(x)
+        dev = x.device
+    if ncol != w.ne0 or (up is not None and up[1:] != w[1:]) or out_dtype not in TYPES:
+        raise ValueError("sizes or types of x, w and up do not fit")
+    offsets = rows = None
+    m = n
+    if group is not None:
+        offsets, rows, m = _index(group.offsets, "offsets"), _index(group.rows, "rows"), group.rows.numel()
+        if group.offsets.numel() != w.nmat + 1:
+            raise ValueError("offsets must be one longer than the stack")
+    y = torch.empty((m, w.ne1), dtype=out_dtype, device=dev)
+    size = gq.gpuq_mxfp4_matmul_work(typ, n, ncol)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    got = gq.gpuq_mxfp4_matmul_dev(typ, ptr, n, ld, w.data.data_ptr(), None if up is None else up.data.data_ptr(),
+                                   w.nmat, w.ne1, w.ne0, offsets, rows, m, TYPES[out_dtype], y.data_ptr(),
+                                   work.data_ptr() if size else None, torch.cuda.current_stream(dev).cuda_stream)
+    if not got:
+        raise ValueError("gpuq_mxfp4_matmul_dev refused %d x %d rows and %d x %d x %d weights" %
+                         (n, ncol, w.nmat, w.ne1, w.ne0))
+    return y
+
+
+def route(gq, logits, k, score="softmax", bias=None, ngroup=1, keep=1, renorm=True, scale=1.0):
+    """the k best experts of every row of logits [n, nexp]: (ids int32 [n, k], weights f32 [n, k]), best first, ties at
+    the lowest index. score 'softmax' or 'sigmoid'; bias f32 [nexp] is added for the choice alone; with ngroup groups
+    only the `keep` best (by their two largest scores) are chosen from; renorm: weights sum to scale."""
+    typ, ptr, n, nexp, ld = _rows(logits)
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(score)
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (nexp,) or not bias.is_contiguous() or
+                             not bias.is_cuda):
+        raise ValueError("bias must be contiguous f32 [%d] on the GPU" % nexp)
+    ids = torch.empty((n, k), dtype=torch.int32, device=logits.device)
+    weights = torch.empty((n, k), dtype=torch.float32, device=logits.device)
+    rc = gq.gpuq_route_dev(typ, ptr, n, ld, nexp, k, int(score == "sigmoid"), None if bias is None else bias.data_ptr(),
+                           ngroup, keep, int(renorm), scale, ids.data_ptr(), weights.data_ptr(), _stream(logits))
+    if rc != 0:
+        raise ValueError("gpuq_route_dev refused %d of %d experts in %d groups (%d)" % (k, nexp, ngroup, rc))
+    return ids, weights
+
+
+def group(gq, ids, nexp):
+    """ids int32 [n, k] -> Group: the n * k assignments sorted by expert, in order within each; ids that name no expert
+    come last, as -1"""
+    ptr = _index(ids, "ids")
+    n, k = ids.shape
+    offsets = torch.empty(nexp + 1, dtype=torch.int32, device=ids.device)
+    rows, slots = torch.empty((2, n * k), dtype=torch.int32, device=ids.device)
+    size = gq.gpuq_route_group_work(n * k, nexp)
+    work = torch.empty(size, dtype=torch.uint8, device=ids.device) if size else None
+    rc = gq.gpuq_route_group_dev(ptr, n, k, nexp, offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
+                                 work.data_ptr() if size else None, _stream(ids))
+    if rc != 0:
+        raise ValueError("gpuq_route_group_dev refused %d x %d ids of %d experts (%d)" % (n, k, nexp, rc))
+    return Group(offsets, rows, slots)
