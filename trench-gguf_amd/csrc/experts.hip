@@ -171,14 +171,18 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
             hipLaunchKernelGGL((k_mx_split<T_F16, 2>), grid, dim3(256), 0, st, d_x, ld, ne0, kp, nx, (uint16_t *)d_work);
         a.x = (const uint8_t *)d_work;
         a.xrow = kp * 2 * pieces;
-        a.kx = kp;
+        a.kx = kp * pieces;
         a.piece = kp * 2;
     }
     const bool glu = d_up != nullptr;
     const int64_t per = m / nmat;                               // rows a group, on average
     if (per <= 16) launch_rows<1>(fp4, glu, a, st);
     else if (per <= 64) launch_rows<4>(fp4, glu, a, st);
-    else if (!launch_tile<2, 2, 4, 4>(fp4, glu, a, st)) return 0;
+    else if (per < 256) {
+        if (!launch_tile<2, 2, 4, 4>(fp4, glu, a, st)) return 0;
+    } else if (!launch_tile<2, 4, 8, 4>(fp4, glu, a, st)) {
+        return 0;
+    }
     return hipGetLastError() == hipSuccess ? (size_t)(m * ne1 * type_size(y_type)) : 0;
 }
 

@@ -265,7 +265,7 @@ DEV void mx_to_lds(const void *g, void *l) {       // 16 bytes a lane to l + 16 
 template <int WM, int WN, int FM, int FN, bool GLU>
 __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
     constexpr int TM = WM * FM * 16, NO = WN * FN * 16 / (GLU ? 2 : 1), NW = WM * WN, LD = TM / 4 / NW;
-    __shared__ __align__(1024) uint8_t xa[TM * 256], xb[TM * 256];
+    __shared__ __align__(1024) uint8_t xs[2 * TM * 256];
     const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, q = lane >> 4, wm = wave / WN, wn = wave % WN;
     const int nt = (int)((a.ne1 + NO - 1) / NO), total = nt * a.mt, per = (total + 7) / 8;
     const int id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
@@ -284,24 +284,25 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
     }
     // where this lane's 16-byte pieces of x come from
     const uint8_t *xp[LD];
-    int at[LD];
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
         const int row = (wave * LD + i) * 4 + (lane >> 4);
         const int64_t r = r0 + row < r1 ? r0 + row : r1 - 1;
         const int64_t j = mx_row(a, r);
         const int p = (lane & 15) ^ (row & 15);
-        at[i] = 4 * (p & 3) + (p >> 2);                     // its piece of the row
-        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * at[i];
+        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * (4 * (p & 3) + (p >> 2));
     }
-    const uint8_t *wp[FN], *sp[FN];
+    uint32_t wo[FN], so[FN];                // codes and scales of this lane's columns, from the tile's first
+    const int64_t n0 = e * a.ne1 + (int64_t)(id % nt) * NO;
+    const int nleft = (int)(a.ne1 - (int64_t)(id % nt) * NO);
+    const uint8_t *wb[2] = {a.w + n0 * (a.np / 2), GLU ? a.u + n0 * (a.np / 2) : nullptr};
+    const uint8_t *sb[2] = {a.ws + n0 * (a.np / 32), GLU ? a.us + n0 * (a.np / 32) : nullptr};
 #pragma unroll
     for (int f = 0; f < FN; ++f) {
-        const bool second = GLU && f >= FN / 2;
-        int64_t n = nb + (GLU ? f % (FN / 2) : f) * 16 + (lane & 15);
-        n = e * a.ne1 + (n < a.ne1 ? n : a.ne1 - 1);
-        wp[f] = (second ? a.u : a.w) + n * (a.np / 2) + 16 * q;
-        sp[f] = (second ? a.us : a.ws) + n * (a.np / 32) + 4 * q;
+        const int n = wn * (NO / WN) + (GLU ? f % (FN / 2) : f) * 16 + (lane & 15);
+        const uint32_t c = (uint32_t)(n < nleft ? n : nleft - 1);
+        wo[f] = c * (uint32_t)(a.np / 2) + 16 * q;
+        so[f] = c * (uint32_t)(a.np / 32) + 4 * q;
     }
     mx_f4 acc[FN][FM];
 #pragma unroll
@@ -309,48 +310,57 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
 #pragma unroll
         for (int g = 0; g < FM; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
     const int steps = a.nk * a.pieces;
+    // a row's pieces follow each other, so a step of x is always 256 bytes; those of the weights start over
     auto stage = [&](int s, uint8_t *buf) {
-        const int p = s / a.nk, c = s - p * a.nk;
-        const int64_t o = p * a.piece + (int64_t)c * 256;
-        const bool tail = (int64_t)c * 128 + 128 > a.kx;
+        if ((int64_t)s * 128 + 128 > a.kx) {        // (the last step, of rows that end inside it)
 #pragma unroll
-        for (int i = 0; i < LD; ++i) {
-            const uint8_t *g = xp[i] + o;
-            if (tail && c * 128 + 8 * at[i] >= a.kx) g = (const uint8_t *)mx_zero;
-            mx_to_lds(g, buf + (wave * LD + i) * 1024);
+            for (int i = 0; i < LD; ++i) {
+                const int p = (lane & 15) ^ (((wave * LD + i) * 4 + (lane >> 4)) & 15);
+                const bool in = (int64_t)s * 128 + 8 * (4 * (p & 3) + (p >> 2)) < a.kx;
+                mx_to_lds(in ? xp[i] : (const uint8_t *)mx_zero, buf + (wave * LD + i) * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < LD; ++i) {
+                mx_to_lds(xp[i], buf + (wave * LD + i) * 1024);
+                xp[i] += 256;
+            }
         }
     };
     uint4 wq[FN];
     uint32_t sc[FN];
-    auto fetch = [&](int s) {
-        const int c = s % a.nk;
+    int c = 0;                              // the weights' next 128
+    auto fetch = [&]() {
 #pragma unroll
         for (int f = 0; f < FN; ++f) {
-            wq[f] = *(const uint4 *)(wp[f] + (int64_t)c * 64);
-            sc[f] = sp[f][(c >> 2) * 16 + (c & 3)];
+            wq[f] = *(const uint4 *)(wb[GLU && f >= FN / 2] + (int64_t)c * 64 + wo[f]);
+            sc[f] = *(sb[GLU && f >= FN / 2] + ((c >> 2) * 16 + (c & 3)) + so[f]);
         }
+        c = c + 1 < a.nk ? c + 1 : 0;
     };
     auto work = [&](const uint8_t *buf, const uint4 (&w)[FN], const uint32_t (&sv)[FN]) {
         const uint8_t *b = buf + (wm * FM * 16 + (lane & 15)) * 256;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            mx_bf8 xv[FM];
+        for (int j = 0; j < 4; ++j) {
+            mx_bf8 xv[FM], wv[FN];
 #pragma unroll
-            for (int g = 0; g < FM; ++g) xv[g] = *(const mx_bf8 *)(b + g * 4096 + (((4 * c + q) ^ (lane & 15)) * 16));
+            for (int g = 0; g < FM; ++g) xv[g] = *(const mx_bf8 *)(b + g * 4096 + (((4 * j + q) ^ (lane & 15)) * 16));
 #pragma unroll
-            for (int f = 0; f < FN; ++f) {
-                const uint32_t cw = c == 0 ? w[f].x : c == 1 ? w[f].y : c == 2 ? w[f].z : w[f].w;
-                const mx_bf8 wv = mx_widen(cw, ffrom(sv[f] << 23));
+            for (int f = 0; f < FN; ++f)
+                wv[f] = mx_widen(j == 0 ? w[f].x : j == 1 ? w[f].y : j == 2 ? w[f].z : w[f].w, ffrom(sv[f] << 23));
 #pragma unroll
-                for (int g = 0; g < FM; ++g)
-                    acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[g], acc[f][g], 0, 0, 0);
-            }
+            for (int g = 0; g < FM; ++g)
+#pragma unroll
+                for (int f = 0; f < FN; ++f)
+                    acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[f], xv[g], acc[f][g], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    stage(0, xa);
-    fetch(0);
+    stage(0, xs);
+    fetch();
     mx_sync();
-    for (int s = 0; s < steps; s += 2) {
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
         uint4 w[FN];
         uint32_t sv[FN];
 #pragma unroll
@@ -359,22 +369,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
             sv[f] = sc[f];
         }
         if (s + 1 < steps) {
-            stage(s + 1, xb);
-            fetch(s + 1);
+            stage(s + 1, xs + ((s + 1) & 1) * (TM * 256));
+            fetch();
         }
-        work(xa, w, sv);
-        mx_sync();
-        if (s + 1 >= steps) break;
-#pragma unroll
-        for (int f = 0; f < FN; ++f) {
-            w[f] = wq[f];
-            sv[f] = sc[f];
-        }
-        if (s + 2 < steps) {
-            stage(s + 2, xa);
-            fetch(s + 2);
-        }
-        work(xb, w, sv);
+        work(xs + (s & 1) * (TM * 256), w, sv);
         mx_sync();
     }
 #pragma unroll
@@ -403,7 +401,7 @@ template <int WM, int WN, int FM, int FN, bool GLU>
 __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile4(MxMulArgs a) {
     constexpr int TM = WM * FM * 16, TN = WN * FN * 16, NO = TN / (GLU ? 2 : 1), NW = WM * WN;
     constexpr int LX = TM / 8 / NW, LW = TN / 8 / NW;
-    __shared__ __align__(1024) uint8_t xa[TM * 128], xb[TM * 128], wa[TN * 128], wb[TN * 128];
+    __shared__ __align__(1024) uint8_t buf[2 * (TM + TN) * 128];
     const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, q = lane >> 4, wm = wave / WN, wn = wave % WN;
     const int nt = (int)((a.ne1 + NO - 1) / NO), total = nt * a.mt, per = (total + 7) / 8;
     const int id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
@@ -460,61 +458,62 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile4(MxMulArgs a) {
     for (int f = 0; f < FN; ++f)
 #pragma unroll
         for (int g = 0; g < FM; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
-    auto stage = [&](int s, uint8_t *x, uint8_t *w) {
+    auto stage = [&](uint8_t *buf) {
 #pragma unroll
-        for (int i = 0; i < LX; ++i) mx_to_lds(xp[i] + (int64_t)s * 128, x + (wave * LX + i) * 1024);
+        for (int i = 0; i < LX; ++i) {
+            mx_to_lds(xp[i], buf + (wave * LX + i) * 1024);
+            xp[i] += 128;
+        }
 #pragma unroll
-        for (int i = 0; i < LW; ++i) mx_to_lds(wp[i] + (int64_t)s * 128, w + (wave * LW + i) * 1024);
+        for (int i = 0; i < LW; ++i) {
+            mx_to_lds(wp[i], buf + TM * 128 + (wave * LW + i) * 1024);
+            wp[i] += 128;
+        }
     };
-    uint32_t xs[FM], ws[FN], xsn[FM], wsn[FN];
+    uint32_t xc[FM], wc[FN], xn[FM], wn_[FN];
     auto scales = [&](int c) {
 #pragma unroll
-        for (int g = 0; g < FM; ++g) xsn[g] = *(const uint32_t *)(xsp[g] + (int64_t)c * 16);
+        for (int g = 0; g < FM; ++g) xn[g] = *(const uint32_t *)(xsp[g] + (int64_t)c * 16);
 #pragma unroll
-        for (int f = 0; f < FN; ++f) wsn[f] = *(const uint32_t *)(wsp[f] + (int64_t)c * 16);
+        for (int f = 0; f < FN; ++f) wn_[f] = *(const uint32_t *)(wsp[f] + (int64_t)c * 16);
     };
     const int sw = (lane >> 1) & 7;
-    auto work = [&](const uint8_t *x, const uint8_t *w, auto half) {
-        constexpr int H = decltype(half)::value;
+    auto work = [&](const uint8_t *buf) {
+        const uint8_t *x = buf + (wm * FM * 16 + (lane & 15)) * 128, *w = buf + (TM + wn * FN * 16 + (lane & 15)) * 128;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint4 xv[FM], wv[FN];
 #pragma unroll
+            for (int f = 0; f < FN; ++f) wv[f] = *(const uint4 *)(w + f * 2048 + ((4 * h + q) ^ sw) * 16);
+#pragma unroll
+            for (int g = 0; g < FM; ++g) xv[g] = *(const uint4 *)(x + g * 2048 + ((4 * h + q) ^ sw) * 16);
+#pragma unroll
             for (int g = 0; g < FM; ++g)
-                xv[g] = *(const uint4 *)(x + ((wm * FM + g) * 16 + (lane & 15)) * 128 + ((4 * h + q) ^ sw) * 16);
 #pragma unroll
-            for (int f = 0; f < FN; ++f)
-                wv[f] = *(const uint4 *)(w + ((wn * FN + f) * 16 + (lane & 15)) * 128 + ((4 * h + q) ^ sw) * 16);
-#pragma unroll
-            for (int f = 0; f < FN; ++f)
-#pragma unroll
-                for (int g = 0; g < FM; ++g)
+                for (int f = 0; f < FN; ++f)
                     acc[f][g] = h == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                             mx_wide(wv[f]), mx_wide(xv[g]), acc[f][g], 4, 4, 2 * H, (int)ws[f], 2 * H,
-                                             (int)xs[g])
+                                             mx_wide(wv[f]), mx_wide(xv[g]), acc[f][g], 4, 4, 0, (int)wc[f], 0, (int)xc[g])
                                        : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                             mx_wide(wv[f]), mx_wide(xv[g]), acc[f][g], 4, 4, 2 * H + 1, (int)ws[f],
-                                             2 * H + 1, (int)xs[g]);
+                                             mx_wide(wv[f]), mx_wide(xv[g]), acc[f][g], 4, 4, 1, (int)wc[f], 1, (int)xc[g]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    const int chunks = (a.nk + 3) / 4, steps = (a.nk + 1) / 2;
-    stage(0, xa, wa);
+    const int steps = (a.nk + 1) / 2;
+    stage(buf);
     scales(0);
     mx_sync();
-    for (int c = 0; c < chunks; ++c) {
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+        // the scales of two steps come as one dword a row
 #pragma unroll
-        for (int g = 0; g < FM; ++g) xs[g] = xsn[g];
+        for (int g = 0; g < FM; ++g) xc[g] = s & 1 ? xn[g] >> 16 : xn[g];
 #pragma unroll
-        for (int f = 0; f < FN; ++f) ws[f] = wsn[f];
-        if (2 * c + 1 < steps) stage(2 * c + 1, xb, wb);
-        work(xa, wa, IntC<0>{});
-        mx_sync();
-        if (2 * c + 1 >= steps) break;
-        if (2 * c + 2 < steps) {
-            stage(2 * c + 2, xa, wa);
-            scales(c + 1);
+        for (int f = 0; f < FN; ++f) wc[f] = s & 1 ? wn_[f] >> 16 : wn_[f];
+        if (s + 1 < steps) {
+            stage(buf + ((s + 1) & 1) * ((TM + TN) * 128));
+            if (s & 1) scales((s + 1) >> 1);
         }
-        work(xb, wb, IntC<1>{});
+        work(buf + (s & 1) * ((TM + TN) * 128));
         mx_sync();
     }
 #pragma unroll
