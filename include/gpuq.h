@@ -152,31 +152,33 @@ size_t gpuq_ldlq(int type, const float *W, const double *H, int64_t h_stride, do
 /* ---- expert layers: MXFP4 rounding, products with stored MXFP4 matrices, routing (no counterpart in the reference,
  * whose calibration pass runs inside llama.cpp or torch). All asynchronous on `stream`; capturable. ----
  *
- * A packed MXFP4 matrix [nrow][n_per_row] holds, with np = n_per_row rounded up to 512, the codes [nrow][np / 2] (value
- * 2i in the low nibble of byte i) and then the scales [nrow][np / 32] (block 4c + q of each 16 at byte 4q + c); its
- * padding is zero. gpuq_mxfp4_packed_bytes: its size, 0 for sizes that no call takes (n_per_row a multiple of 32, at most
- * 2^24). A stack of nmat matrices is one packed matrix of nmat * ne1 rows. */
-size_t gpuq_mxfp4_packed_bytes(int64_t nrow, int64_t n_per_row);
+ * MXFP4 data has three forms. 0: ggml's 17-byte blocks. For products rows are padded to np = n_per_row rounded up to 512
+ * with zeros: 1 rows (what is multiplied; any row can be picked): codes [nrow][np / 2], value 2i in the low nibble of byte
+ * i, then scales [np / 512][nrow][16], block 4c + q of the 16 at byte 4q + c. 2 tiles (stored matrices, each padded to
+ * whole strips of 16 rows): codes [strip][np / 128][64][16], piece 16q + r the codes of row r's block q, then scales
+ * [strip][np / 512][64][4], byte c of piece 16q + r row r's block 4c + q.
+ * gpuq_mxfp4_bytes: the bytes of nmat matrices of a form, 0 for sizes that no call takes (n_per_row a multiple of 32, at
+ * most 2^24; at most 2^30 strips). */
+size_t gpuq_mxfp4_bytes(int form, int64_t nmat, int64_t nrow, int64_t n_per_row);
 
-/* Rounds rows to MXFP4: d_src F32 / F16 / BF16 [nrow][n_per_row], ld elements from row to row (rows 16-byte aligned) ->
- * d_dst, packed (1) or ggml's 17-byte blocks (0), and, where d_values is not NULL, the rounded values as BF16
- * [nrow][n_per_row] (exact). A block of 32 shares 2^(floor(log2(largest)) - 2), its exponent clamped to what e8m0 holds;
- * a value becomes the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (a tie the smaller, past 6 becomes 6, no negative
- * zero). A NaN becomes 0, an infinity 6 * 2^125. src_type MXFP4 (ggml's blocks, ld = n_per_row) with packed 1 lays
- * stored blocks out packed, bit for bit. d_dst, d_values and d_src (but MXFP4's) 16-byte aligned. Returns the bytes of
- * d_dst, 0 on an error. */
-size_t gpuq_mxfp4_quantize_dev(int src_type, const void *d_src, int64_t nrow, int64_t n_per_row, int64_t ld, int packed,
-                               void *d_dst, void *d_values, void *stream);
+/* Rounds rows to MXFP4: d_src F32 / F16 / BF16 [nmat][nrow][n_per_row], ld elements from row to row (rows 16-byte
+ * aligned) -> d_dst in the form, and, where d_values is not NULL, the rounded values as BF16 [nmat][nrow][n_per_row]
+ * (exact). A block of 32 shares 2^(floor(log2(largest)) - 2), its exponent clamped to what e8m0 holds; a value becomes the
+ * nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (a tie the smaller, past 6 becomes 6, no negative zero). A NaN becomes 0,
+ * an infinity 6 * 2^125. src_type MXFP4 (ggml's blocks, ld = n_per_row) with form 1 or 2 lays stored blocks out, bit for
+ * bit. d_dst, d_values and d_src (but MXFP4's) 16-byte aligned. Returns the bytes of d_dst, 0 on an error. */
+size_t gpuq_mxfp4_quantize_dev(int src_type, const void *d_src, int64_t nmat, int64_t nrow, int64_t n_per_row, int64_t ld,
+                               int form, void *d_dst, void *d_values, void *stream);
 
 /* The scratch bytes gpuq_mxfp4_matmul_dev needs at d_work for nx rows of x_type (0 for BF16 and MXFP4: NULL will do) */
 size_t gpuq_mxfp4_matmul_work(int x_type, int64_t nx, int64_t ne0);
 
-/* Products of rows with packed MXFP4 matrices d_w [nmat][ne1][ne0]: y[r] = x[d_rows[r]] w[e]^T for the rows
+/* Products of rows with MXFP4 matrices d_w [nmat][ne1][ne0] (tiles): y[r] = x[d_rows[r]] w[e]^T for the rows
  * d_offsets[e] <= r < d_offsets[e + 1] of matrix e (int32, device; nmat 1: d_offsets may be NULL, all m rows). d_rows NULL:
- * x[r]. With d_up (packed, the same sizes) SwiGLU: y = g / (1 + exp(-g)) * u, g of d_w and u of d_up. x_type: BF16, F16,
- * F32 [nx][ld] (rows 16-byte aligned; no bit of x or w is rounded away, sums in f32) or packed MXFP4 (39, ld = ne0).
+ * x[r]. With d_up (tiles, the same sizes) SwiGLU: y = g / (1 + exp(-g)) * u, g of d_w and u of d_up. x_type: BF16, F16,
+ * F32 [nx][ld] (rows 16-byte aligned; no bit of x or w is rounded away, sums in f32) or MXFP4 rows (39, ld = ne0).
  * y_type F32, F16 or BF16: d_y [m][ne1]. A row that no matrix has (r >= d_offsets[nmat]) or whose d_rows names no row of x
- * is zero. A scale of 255 is NaN (unlike in ggml's to_float, which takes it for 2^128). At most 65534 matrices and 2^30
+ * is zero. A scale of 255 is NaN (ggml's to_float takes it for 2^128). At most 65534 matrices and 2^30
  * rows; pointers 16-byte aligned (d_offsets, d_rows 4). Returns the bytes of d_y, 0 on an error. */
 size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx, int64_t ld, const void *d_w, const void *d_up,
                              int64_t nmat, int64_t ne1, int64_t ne0, const int32_t *d_offsets, const int32_t *d_rows,

@@ -9,10 +9,11 @@ def lib():
 
 
 def test_sizes(lib):
-    assert lib.gpuq_mxfp4_packed_bytes(2, 512) == 2 * (256 + 16)
-    assert lib.gpuq_mxfp4_packed_bytes(5, 32) == 5 * (256 + 16)
-    assert lib.gpuq_mxfp4_packed_bytes(1, 7168) == 7168 * 17 // 32
-    assert [lib.gpuq_mxfp4_packed_bytes(*a) for a in ((0, 32), (1, 0), (1, 33), (-1, 32), (1, 1 << 25))] == [0] * 5
+    assert [lib.gpuq_mxfp4_bytes(f, 2, 3, 512) for f in (0, 1, 2)] == [6 * 272, 6 * 272, 32 * 272]
+    assert [lib.gpuq_mxfp4_bytes(f, 1, 5, 32) for f in (0, 1, 2)] == [5 * 17, 5 * 272, 16 * 272]
+    assert lib.gpuq_mxfp4_bytes(2, 256, 2048, 7168) == 256 * 2048 * 7168 * 17 // 32
+    assert [lib.gpuq_mxfp4_bytes(*a) for a in ((0, 1, 0, 32), (1, 0, 1, 32), (2, 1, 1, 33), (1, 1, -1, 32), (3, 1, 1, 32),
+                                               (-1, 1, 1, 32), (0, 1, 1, 1 << 25), (2, 1 << 20, 1 << 20, 32))] == [0] * 8
     assert [lib.gpuq_mxfp4_matmul_work(t, 10, 100 * 32) for t in (0, 1, 30, 39)] == [10 * 3200 * 6, 10 * 3200 * 4, 0, 0]
     assert lib.gpuq_mxfp4_matmul_work(0, 3, 32) == 3 * 128 * 6
     assert lib.gpuq_route_group_work(2048, 64) == 0 and lib.gpuq_route_group_work(2049, 64) == 2 * 64 * 4
@@ -21,7 +22,7 @@ def test_sizes(lib):
 def test_nothing_runs_before_init(lib):
     if lib.gpuq_can_dequantize_type(23) == 1:
         pytest.skip("the library was initialized earlier in this process (GPU tests ran first)")
-    assert lib.gpuq_mxfp4_quantize_dev(0, 4096, 1, 32, 32, 0, 4096, None, None) == 0
+    assert lib.gpuq_mxfp4_quantize_dev(0, 4096, 1, 1, 32, 32, 0, 4096, None, None) == 0
     assert lib.gpuq_mxfp4_matmul_dev(30, 4096, 1, 32, 4096, None, 1, 1, 32, None, None, 1, 0, 4096, None, None) == 0
     assert lib.gpuq_route_dev(0, 4096, 1, 8, 8, 2, 0, None, 1, 1, 1, 1.0, 4096, 4096, None) == 1
     assert lib.gpuq_route_group_dev(4096, 1, 2, 8, 4096, 4096, 4096, None, None) == 1

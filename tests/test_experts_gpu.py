@@ -65,12 +65,27 @@ def as_blocks(code, e):
     return np.concatenate((e[..., None], c[:, :, 0] | (c[:, :, 1] << 4)), axis=2).reshape(n, -1).astype(np.uint8)
 
 
-def from_packed(data, n, ncol):
-    """(codes, exponents, whether the padding is zero) of a packed tensor's bytes"""
+def from_rows(data, n, ncol):
+    """(codes, exponents, whether the padding is zero) of MXFP4 rows' bytes"""
     npad = (ncol + 511) // 512 * 512
     c = data[:n * npad // 2].reshape(n, npad // 2)
-    s = data[n * npad // 2:].reshape(n, npad // 512, 4, 4).transpose(0, 1, 3, 2).reshape(n, npad // 32)
-    codes = np.stack((c & 15, c >> 4), axis=2).reshape(n, npad)
+    s = data[n * npad // 2:].reshape(npad // 512, n, 4, 4).transpose(1, 0, 3, 2).reshape(n, npad // 32)
+    return unpadded(np.stack((c & 15, c >> 4), axis=2).reshape(n, npad), s, n, ncol)
+
+
+def from_tiles(data, nmat, nrow, ncol):
+    """the same of matrices laid out in tiles, their rows one after the other"""
+    npad, strips = (ncol + 511) // 512 * 512, (nrow + 15) // 16
+    size = nmat * strips * 8 * npad
+    c = data[:size].reshape(nmat * strips, npad // 128, 4, 16, 16).transpose(0, 3, 1, 2, 4).reshape(-1, npad // 2)
+    s = data[size:].reshape(nmat * strips, npad // 512, 4, 16, 4).transpose(0, 3, 1, 4, 2).reshape(-1, npad // 32)
+    c = np.stack((c & 15, c >> 4), axis=2).reshape(nmat, strips * 16, npad)
+    s = s.reshape(nmat, strips * 16, npad // 32)
+    codes, e, clean = unpadded(c[:, :nrow].reshape(-1, npad), s[:, :nrow].reshape(-1, npad // 32), nmat * nrow, ncol)
+    return codes, e, clean and not c[:, nrow:].any() and not s[:, nrow:].any()
+
+
+def unpadded(codes, s, n, ncol):
     return codes[:, :ncol], s[:, :ncol // 32], not codes[:, ncol:].any() and not s[:, ncol // 32:].any()
 
 
@@ -135,20 +150,25 @@ def edge_rows(rng, ncol):
     return x
 
 
-@pytest.mark.parametrize("packed", [False, True], ids=["blocks", "packed"])
+@pytest.mark.parametrize("form", ["blocks", "rows", "tiles"])
 @pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("ncol", [32, 96, 512, 544, 1760])
-def test_quantize_matches_the_nearest_levels(gq, ex, src, ncol, packed):
+def test_quantize_matches_the_nearest_levels(gq, ex, src, ncol, form):
     torch = torch_()
     x = torch.from_numpy(edge_rows(np.random.default_rng(ncol), ncol)).to(dtype(src))
     x = torch.nan_to_num(x, posinf=6e4, neginf=-6e4) if src == "f16" else x
     x = torch.nan_to_num(x, posinf=3e38, neginf=-3e38) if src == "bf16" else x
     code, e = round_blocks(x.double().numpy())
     d = x.cuda()
-    if packed:
+    if form == "rows":
         p, values = ex.quantize(gq, d, values=True)
-        c, s, clean = from_packed(p.data.cpu().numpy(), len(x), ncol)
+        c, s, clean = from_rows(p.data.cpu().numpy(), len(x), ncol)
         assert clean and np.array_equal(c, code) and np.array_equal(s, e)
+    elif form == "tiles":
+        p, values = ex.quantize_weights(gq, d.view(2, 7, ncol), values=True)
+        c, s, clean = from_tiles(p.data.cpu().numpy(), 2, 7, ncol)
+        assert clean and np.array_equal(c, code) and np.array_equal(s, e)
+        values = values.view(14, ncol)
     else:
         blocks, values = ex.quantize_blocks(gq, d, values=True)
         assert np.array_equal(blocks.cpu().numpy(), as_blocks(code, e))
@@ -167,8 +187,8 @@ def test_quantize_takes_strided_rows_and_many_blocks(gq, ex, src):
     assert np.array_equal(f64(values), code_values(code, e))
     size = 77 * 23 * 17
     out = torch.full((size + 64,), 0xA5, dtype=torch.uint8, device="cuda")
-    got = gq.gpuq_mxfp4_quantize_dev(F32 if src == "f32" else BF16, x.data_ptr(), 77, 736, 3 * 736, 0, out.data_ptr(), None,
-                                     torch.cuda.current_stream().cuda_stream)
+    got = gq.gpuq_mxfp4_quantize_dev(F32 if src == "f32" else BF16, x.data_ptr(), 7, 11, 736, 3 * 736, 0,
+                                     out.data_ptr(), None, torch.cuda.current_stream().cuda_stream)
     assert got == size and np.array_equal(out[:size].cpu().numpy(), as_blocks(code, e).ravel())
     assert bool((out[size:] == 0xA5).all())
 
@@ -202,7 +222,14 @@ def test_blocks_read_back_as_the_library_reads_them(gq, ex):
 def test_pack_keeps_every_bit(gq, ex, ne0):
     code, e = random_weights(np.random.default_rng(ne0), 3, 37, ne0, 0, 256)
     p = packed_weights(ex, gq, code, e, 3)
-    c, s, clean = from_packed(p.data.cpu().numpy(), 3 * 37, ne0)
+    c, s, clean = from_tiles(p.data.cpu().numpy(), 3, 37, ne0)
+    assert clean and np.array_equal(c, code) and np.array_equal(s, e)
+    blocks = torch_().from_numpy(as_blocks(code, e)).cuda()
+    size = gq.gpuq_mxfp4_bytes(1, 3, 37, ne0)
+    out = torch_().empty(size, dtype=torch_().uint8, device="cuda")
+    assert gq.gpuq_mxfp4_quantize_dev(MXFP4, blocks.data_ptr(), 3, 37, ne0, ne0, 1, out.data_ptr(), None,
+                                      torch_().cuda.current_stream().cuda_stream) == size
+    c, s, clean = from_rows(out.cpu().numpy(), 3 * 37, ne0)
     assert clean and np.array_equal(c, code) and np.array_equal(s, e)
 
 
@@ -363,7 +390,7 @@ def test_products_past_32_bits(gq, ex):
     rng = np.random.default_rng(0)
     code, e = random_weights(rng, 1, ne1, ne0)
     one = torch.from_numpy(as_blocks(code, e)).cuda()
-    size = gq.gpuq_mxfp4_packed_bytes(nmat * ne1, ne0)
+    size = gq.gpuq_mxfp4_bytes(2, nmat, ne1, ne0)
     assert size > 1 << 32
     data = torch.zeros(size, dtype=torch.uint8, device="cuda")
     p = ex.pack(gq, one, 1, ne1, ne0).data
@@ -548,20 +575,16 @@ def test_refusals(gq, ex):
     out = torch.zeros(1 << 18, dtype=torch.uint8, device="cuda")
     p, o = x.data_ptr(), out.data_ptr()
     q = gq.gpuq_mxfp4_quantize_dev
-    assert q(BF16, p, 4, 512, 512, 0, o, None, st) == 4 * 16 * 17
-    assert q(BF16, p, 0, 512, 512, 0, o, None, st) == 0
-    assert q(BF16, p, 4, 500, 512, 0, o, None, st) == 0         # not whole blocks
-    assert q(BF16, p, 4, 512, 480, 0, o, None, st) == 0         # rows overlap
-    assert q(BF16, p, 4, 512, 516, 0, o, None, st) == 0         # unaligned rows
-    assert q(BF16, p + 2, 4, 512, 512, 0, o, None, st) == 0
-    assert q(BF16, p, 4, 512, 512, 0, o + 1, None, st) == 0
-    assert q(BF16, p, 4, 512, 512, 0, o, o + 4, st) == 0
-    assert q(BF16, p, 4, 512, 512, 2, o, None, st) == 0
-    assert q(Q8_0, p, 4, 512, 512, 0, o, None, st) == 0         # not a float type
-    assert q(MXFP4, p, 4, 512, 512, 0, o, None, st) == 0        # blocks to blocks
-    assert q(BF16, None, 4, 512, 512, 0, o, None, st) == 0
-    assert gq.gpuq_mxfp4_packed_bytes(1, 33) == 0 and gq.gpuq_mxfp4_packed_bytes(0, 32) == 0
-    assert gq.gpuq_mxfp4_packed_bytes(3, 544) == 3 * 1024 * 17 // 32
+    good = [BF16, p, 2, 2, 512, 512, 0, o, None, st]
+    assert q(*good) == 4 * 16 * 17
+    for at, bad in ((0, Q8_0), (0, MXFP4), (1, None), (1, p + 2), (2, 0), (3, 0), (3, -1), (4, 500), (4, 0), (5, 480),
+                    (5, 516), (6, 3), (6, -1), (7, None), (7, o + 1), (8, o + 4)):
+        args = list(good)
+        args[at] = bad
+        assert q(*args) == 0, (at, bad)
+    assert q(MXFP4, p, 2, 2, 512, 544, 1, o, None, st) == 0
+    assert gq.gpuq_mxfp4_bytes(1, 1, 1, 33) == 0 and gq.gpuq_mxfp4_bytes(2, 1, 0, 32) == 0
+    assert gq.gpuq_mxfp4_bytes(1, 1, 3, 544) == 3 * 1024 * 17 // 32 and gq.gpuq_mxfp4_bytes(2, 2, 17, 32) == 64 * 272
     mm = gq.gpuq_mxfp4_matmul_dev
     good = [BF16, p, 64, 512, o, None, 1, 32, 512, None, None, 64, F32, o, None, st]
     for at, bad in ((0, Q8_0), (1, None), (1, p + 2), (2, 0), (3, 500), (4, None), (4, o + 8), (5, o + 8), (6, 0), (6, 2),

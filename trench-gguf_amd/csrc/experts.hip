@@ -3,6 +3,8 @@
 // conventions, in include/gpuq.h).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "mxfp4.cuh"
 #include "mxmul.cuh"
 #include "route.cuh"
@@ -17,22 +19,25 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int64_t MAX_BLOCKS = (int64_t)1 << 30;                // of a launch (32-bit block numbers)
 constexpr int64_t MAX_ROWS = (int64_t)1 << 30;
 
-int64_t packed_bytes(int64_t nrow, int64_t n) { return nrow * (mx_padded(n) / 2 + mx_padded(n) / 32); }
-
 // a row length of whole blocks whose padded rows stay countable
 bool cols_ok(int64_t n) { return n > 0 && n % 32 == 0 && n <= (int64_t)1 << 24; }
+int64_t strips_of(int64_t nrow) { return (nrow + 15) / 16; }
+// rows of the layout, the padding of tiles among them
+int64_t stored_rows(int64_t nmat, int64_t nrow, int form) {
+    return form == MX_TILES ? nmat * strips_of(nrow) * 16 : nmat * nrow;
+}
 
-template <int SRC> void launch_quantize(bool packed, const MxQuantArgs &p, hipStream_t st) {
+template <int SRC> void launch_quantize(int form, const MxQuantArgs &p, hipStream_t st) {
     const unsigned grid = (unsigned)((p.nblk + MX_U * 64 - 1) / (MX_U * 64));
-    if (packed) hipLaunchKernelGGL((k_mx_quantize<SRC, true>), dim3(grid), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((k_mx_quantize<SRC, false>), dim3(grid), dim3(256), 0, st, p);
+    if (form == MX_ROWS) hipLaunchKernelGGL((k_mx_quantize<SRC, MX_ROWS>), dim3(grid), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_mx_quantize<SRC, MX_BLOCKS>), dim3(grid), dim3(256), 0, st, p);
 }
 
 int pieces_of(int x_type) { return x_type == T_F32 ? 3 : x_type == T_F16 ? 2 : 1; }
 int64_t round128(int64_t n) { return (n + 127) / 128 * 128; }
 
 template <int MF> void launch_rows(bool fp4, bool glu, const MxMulArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)((a.ne1 + 15) / 16), (unsigned)(a.offsets ? a.nmat + 1 : 1));
+    const dim3 grid((unsigned)a.strips, (unsigned)(a.offsets ? a.nmat + 1 : 1));
 #define MX_ROWS(F, G) hipLaunchKernelGGL((k_mx_rows<F, MF, G>), grid, dim3(512), 0, st, a)
     if (fp4) {
         if (glu) MX_ROWS(true, true);
@@ -51,13 +56,15 @@ template <int WM, int WN, int FM, int FN> bool launch_tile(bool fp4, bool glu, M
     if (nt * mt >= ((int64_t)1 << 30)) return false;
     a.mt = (int)mt;
     const dim3 grid((unsigned)((nt * mt + 7) / 8 * 8)), block(WM * WN * 64);
+#define MX_TILE(F, G) hipLaunchKernelGGL((k_mx_tile<F, WM, WN, FM, FN, G>), grid, block, 0, st, a)
     if (fp4) {
-        if (glu) hipLaunchKernelGGL((k_mx_tile4<WM, WN, FM, FN, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((k_mx_tile4<WM, WN, FM, FN, false>), grid, block, 0, st, a);
+        if (glu) MX_TILE(true, true);
+        else MX_TILE(true, false);
     } else {
-        if (glu) hipLaunchKernelGGL((k_mx_tile<WM, WN, FM, FN, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((k_mx_tile<WM, WN, FM, FN, false>), grid, block, 0, st, a);
+        if (glu) MX_TILE(false, true);
+        else MX_TILE(false, false);
     }
+#undef MX_TILE
     return true;
 }
 
@@ -74,46 +81,70 @@ template <int SRC> bool launch_route(const RouteArgs &a, hipStream_t st) {
 
 }  // namespace
 
-extern "C" size_t gpuq_mxfp4_packed_bytes(int64_t nrow, int64_t n_per_row) {
-    if (nrow <= 0 || nrow >= ((int64_t)1 << 40) / 32 || !cols_ok(n_per_row)) return 0;
-    return (size_t)packed_bytes(nrow, n_per_row);
+extern "C" size_t gpuq_mxfp4_bytes(int form, int64_t nmat, int64_t nrow, int64_t n_per_row) {
+    if (form < MX_BLOCKS || form > MX_TILES || nmat <= 0 || nrow <= 0 || nmat > MAX_ROWS || nrow > MAX_ROWS ||
+        nmat * strips_of(nrow) > MAX_ROWS || !cols_ok(n_per_row))
+        return 0;
+    return (size_t)(stored_rows(nmat, nrow, form) * ((form == MX_BLOCKS ? n_per_row : mx_padded(n_per_row)) / 32 * 17));
 }
 
-extern "C" size_t gpuq_mxfp4_quantize_dev(int src_type, const void *d_src, int64_t nrow, int64_t n_per_row, int64_t ld,
-                                          int packed, void *d_dst, void *d_values, void *stream) {
-    if (gq_device() < 0 || !d_src || !d_dst || !gpuq_mxfp4_packed_bytes(nrow, n_per_row)) return 0;
-    if (packed != 0 && packed != 1) return 0;
-    if (!aligned16(d_dst) || !aligned16(d_values)) return 0;
+extern "C" size_t gpuq_mxfp4_quantize_dev(int src_type, const void *d_src, int64_t nmat, int64_t nrow, int64_t n_per_row,
+                                          int64_t ld, int form, void *d_dst, void *d_values, void *stream) {
+    const size_t size = gpuq_mxfp4_bytes(form, nmat, nrow, n_per_row);
+    if (gq_device() < 0 || !d_src || !d_dst || !size || !aligned16(d_dst) || !aligned16(d_values)) return 0;
     if (src_type == T_MXFP4) {
-        if (!packed || ld != n_per_row) return 0;
+        if (form == MX_BLOCKS || ld != n_per_row) return 0;
     } else if (!float_type(src_type) || ld < n_per_row || ld > ((int64_t)1 << 40) || !aligned16(d_src) ||
                ld * type_size(src_type) % 16) {
         return 0;
     }
-    const int64_t nb = n_per_row / 32, stored = packed ? mx_padded(n_per_row) / 32 : nb, rows_max = MAX_BLOCKS / stored;
-    uint8_t *dst = (uint8_t *)d_dst, *scales = dst + nrow * stored * 16;
-    for (int64_t r = 0; r < nrow; r += rows_max) {
-        const int64_t n = nrow - r < rows_max ? nrow - r : rows_max;
-        MxQuantArgs p;
+    const hipStream_t st = (hipStream_t)stream;
+    const int64_t nb = n_per_row / 32, np = mx_padded(n_per_row), rows = nmat * nrow;
+    MxQuantArgs p = {};
+    p.ld = ld;
+    p.ncol = n_per_row;
+    p.nb = (uint32_t)nb;
+    if (form == MX_TILES) {
+        const int64_t strips = strips_of(nrow);
+        p.src = d_src;
+        p.nrow = nrow;
+        p.dst = (uint8_t *)d_dst;
+        p.scales = p.dst + nmat * strips * 8 * np;
+        p.values = (uint16_t *)d_values;
+        p.row = mx_div((uint32_t)strips);
+        for (int64_t s = 0; s < nmat * strips; s += 65535) {
+            const dim3 grid((unsigned)(np / 512), (unsigned)std::min<int64_t>(65535, nmat * strips - s));
+            p.row0 = s;
+            switch (src_type) {
+                case T_F32: hipLaunchKernelGGL(k_mx_tiles<T_F32>, grid, dim3(256), 0, st, p); break;
+                case T_F16: hipLaunchKernelGGL(k_mx_tiles<T_F16>, grid, dim3(256), 0, st, p); break;
+                case T_BF16: hipLaunchKernelGGL(k_mx_tiles<T_BF16>, grid, dim3(256), 0, st, p); break;
+                default: hipLaunchKernelGGL(k_mx_tiles<T_MXFP4>, grid, dim3(256), 0, st, p);
+            }
+            if (hipGetLastError() != hipSuccess) return 0;
+        }
+        return size;
+    }
+    const int64_t stored = form == MX_ROWS ? np / 32 : nb, rows_max = MAX_BLOCKS / stored;
+    p.nrow = rows;
+    p.row = mx_div((uint32_t)stored);
+    p.scales = form == MX_ROWS ? (uint8_t *)d_dst + rows * stored * 16 : nullptr;
+    for (int64_t r = 0; r < rows; r += rows_max) {
         p.src = (const uint8_t *)d_src + (src_type == T_MXFP4 ? r * nb * 17 : r * ld * type_size(src_type));
-        p.ld = ld;
-        p.dst = dst + r * stored * (packed ? 16 : 17);
-        p.scales = packed ? scales + r * stored : nullptr;
+        p.dst = (uint8_t *)d_dst + r * stored * (form == MX_ROWS ? 16 : 17);
         p.values = d_values ? (uint16_t *)d_values + r * n_per_row : nullptr;
-        p.ncol = n_per_row;
-        p.nblk = (uint32_t)(n * stored);
-        p.nb = (uint32_t)nb;
-        p.row = mx_div((uint32_t)stored);
+        p.row0 = r;
+        p.nblk = (uint32_t)(std::min(rows_max, rows - r) * stored);
         switch (src_type) {
-            case T_F32: launch_quantize<T_F32>(packed != 0, p, (hipStream_t)stream); break;
-            case T_F16: launch_quantize<T_F16>(packed != 0, p, (hipStream_t)stream); break;
-            case T_BF16: launch_quantize<T_BF16>(packed != 0, p, (hipStream_t)stream); break;
-            default: hipLaunchKernelGGL((k_mx_quantize<T_MXFP4, true>), dim3((unsigned)((p.nblk + MX_U * 64 - 1) / (MX_U * 64))),
-                                        dim3(256), 0, (hipStream_t)stream, p);
+            case T_F32: launch_quantize<T_F32>(form, p, st); break;
+            case T_F16: launch_quantize<T_F16>(form, p, st); break;
+            case T_BF16: launch_quantize<T_BF16>(form, p, st); break;
+            default: hipLaunchKernelGGL((k_mx_quantize<T_MXFP4, MX_ROWS>), dim3((p.nblk + MX_U * 64 - 1) / (MX_U * 64)),
+                                        dim3(256), 0, st, p);
         }
         if (hipGetLastError() != hipSuccess) return 0;
     }
-    return (size_t)(nrow * stored * 17);
+    return size;
 }
 
 extern "C" size_t gpuq_mxfp4_matmul_work(int x_type, int64_t nx, int64_t ne0) {
@@ -127,7 +158,7 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
                                         void *d_y, void *d_work, void *stream) {
     const bool fp4 = x_type == T_MXFP4;
     if (gq_device() < 0 || !d_x || !d_w || !d_y || (!fp4 && !float_type(x_type)) || !float_type(y_type)) return 0;
-    if (nmat <= 0 || nmat > 65534 || ne1 <= 0 || ne1 > MAX_ROWS || !cols_ok(ne0) || nx <= 0 || nx > MAX_ROWS || m <= 0 ||
+    if (nmat <= 0 || nmat > 65534 || nmat * strips_of(ne1) > MAX_ROWS || ne1 <= 0 || ne1 > MAX_ROWS || !cols_ok(ne0) || nx <= 0 || nx > MAX_ROWS || m <= 0 ||
         m > MAX_ROWS || (nmat > 1 && !d_offsets) || (!d_rows && m > nx))
         return 0;
     if (!aligned16(d_x) || !aligned16(d_w) || !aligned16(d_up) || !aligned16(d_y) || ((uintptr_t)d_offsets & 3) ||
@@ -137,7 +168,7 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
     const int pieces = pieces_of(x_type);
     if (pieces > 1 && (!d_work || !aligned16(d_work))) return 0;
     const hipStream_t st = (hipStream_t)stream;
-    const int64_t np = mx_padded(ne0), wcodes = nmat * ne1 * (np / 2);
+    const int64_t np = mx_padded(ne0), strips = strips_of(ne1), wcodes = nmat * strips * 8 * np;
     MxMulArgs a = {};
     a.nx = nx;
     a.w = (const uint8_t *)d_w;
@@ -146,7 +177,8 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
     a.us = d_up ? a.u + wcodes : nullptr;
     a.nmat = nmat;
     a.ne1 = ne1;
-    a.np = np;
+    a.strips = strips;
+    a.nc = (int)(np / 512);
     a.nk = (int)(round128(ne0) / 128);
     a.offsets = d_offsets;
     a.rows = d_rows;
@@ -172,7 +204,6 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
         a.x = (const uint8_t *)d_work;
         a.xrow = kp * 2 * pieces;
         a.kx = kp * pieces;
-        a.piece = kp * 2;
     }
     const bool glu = d_up != nullptr;
     const int64_t per = m / nmat;                               // rows a group, on average

@@ -7,11 +7,15 @@
 // division by the scale is a multiplication by a power of two and so exact. NaN counts as zero, an infinity as the
 // largest magnitude there is.
 //
-// Packed layout of an [nrow][n_per_row] matrix, np = n_per_row rounded up to 512:
-//   codes   [nrow][np / 2] bytes, value 2i in the low nibble of byte i and 2i + 1 in the high one;
-//   scales  [nrow][np / 32] bytes, after all the codes: block 4c + q of each 16 at byte 4q + c, so that lane group q of
-//           a 16 x 16 x 128 product finds the scales of four products running in one dword.
-// The padding is zero codes with zero scales. A row's codes are whole 256-byte pieces, so the products need no tails.
+// Two layouts for products, of rows padded to np = n_per_row rounded up to 512, the padding zero codes at zero scales:
+//   rows (what products multiply; any row can be picked): codes [nrow][np / 2] bytes, value 2i in the low nibble of byte
+//     i; then scales [np / 512][nrow][16], block 4c + q of the 16 at byte 4q + c.
+//   tiles (stored matrices, each padded to whole strips of 16 rows): codes [strip][np / 128][64][16], piece 16q + r the
+//     codes of row r's block q of the 128; then scales [strip][np / 512][64][4], byte c of piece 16q + r row r's block
+//     4c + q. A strip's 128 columns are one kilobyte in the order in which the lanes of a 16 x 16 x 128 product take
+//     them, so a wave loads its operand from 8 whole lines (from rows 3584 bytes apart the same bytes came as 16 half
+//     lines, and the products waited for the loads: 4096 x 2048 x 7168 took 183 us with the rows of x left out and 135
+//     with these loads left out too).
 #pragma once
 #include "common.cuh"
 
@@ -95,16 +99,57 @@ struct MxQuantArgs {
     int64_t ld;                 // source elements from row to row (MXFP4: unused, rows are whole blocks)
     uint8_t *dst, *scales;      // blocks, or codes and scales
     uint16_t *values;           // BF16, or null
-    int64_t ncol;
-    uint32_t nblk, nb;          // blocks this launch makes, and those of a row that hold values
-    MxDiv row;                  // blocks of a row as stored (nb, or with the padding)
+    int64_t ncol, nrow;         // of the whole call (rows), of a matrix (tiles)
+    int64_t row0;               // the launch's first row (rows)
+    uint32_t nblk, nb;          // blocks of this launch, and those of a row that hold values
+    MxDiv row;                  // blocks of a row as stored (nb, or with the padding); tiles: strips of a matrix
 };
 
-// four lanes a block, 8 values a lane, MX_U blocks a lane
+enum { MX_BLOCKS = 0, MX_ROWS = 1, MX_TILES = 2 };
+
+// 8 values of a block (quarter a of it): the source's, zero where the block holds none
+template <int SRC> DEV void mx_source(const MxQuantArgs &p, int64_t row, uint32_t col, bool real, int a, float (&v)[8],
+                                      uint32_t (&raw)[3]) {
+    if (SRC == T_MXFP4) {
+        const uint8_t *blk = (const uint8_t *)p.src + (real ? row * p.nb + col : 0) * 17;
+        raw[2] = blk[0];
+        __builtin_memcpy(&raw[0], blk + 1 + 8 * (a & 1), 8);
+        if (!real) raw[0] = raw[1] = raw[2] = 0;
+    } else {
+        mx_load8<SRC>(p.src, (real ? row * p.ld + (int64_t)col * 32 : 0) + 8 * a, v);
+        if (!real) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        }
+    }
+}
+// their codes and the block's scale exponent (over the 4 lanes that share it)
+template <int SRC> DEV uint32_t mx_encode(int a, const float (&v)[8], const uint32_t (&raw)[3], uint32_t &e) {
+    uint32_t codes = 0;
+    if (SRC == T_MXFP4) {
+        const int sh = 4 * (a >> 1);
+        codes = mx_gather((raw[0] >> sh) & 0x0f0f0f0fu) | (mx_gather((raw[1] >> sh) & 0x0f0f0f0fu) << 16);
+        e = raw[2];
+    } else {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));             // (a NaN is passed over)
+        m = fmaxf(m, ffrom(mx_quad<0xB1>(fbits(m))));
+        m = fmaxf(m, ffrom(mx_quad<0x4E>(fbits(m))));
+        const int x = (int)(fbits(m) >> 23) - 2;
+        e = (uint32_t)(x < 0 ? 0 : x > 252 ? 252 : x);
+        const float inv = ffrom((254 - e) << 23);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) codes |= mx_code(v[j], inv) << (4 * j);
+    }
+    return codes;
+}
+
+// blocks and rows: four lanes a block, 8 values a lane, MX_U blocks a lane
 #define MX_U 4
-template <int SRC, bool PACKED>
+template <int SRC, int FORM>
 __global__ __launch_bounds__(256) void k_mx_quantize(MxQuantArgs p) {
-    __shared__ __align__(16) uint8_t out[PACKED ? 16 : MX_U * 64 * 17];
+    __shared__ __align__(16) uint8_t out[FORM == MX_ROWS ? 16 : MX_U * 64 * 17];
     const int tid = threadIdx.x, a = tid & 3;
     const uint32_t b0 = blockIdx.x * (MX_U * 64) + (tid >> 2);
     float v[MX_U][8];
@@ -114,48 +159,19 @@ __global__ __launch_bounds__(256) void k_mx_quantize(MxQuantArgs p) {
         const uint32_t b = b0 + 64 * u < p.nblk ? b0 + 64 * u : p.nblk - 1;
         row[u] = p.row.div(b);
         col[u] = b - row[u] * p.row.d;
-        const bool real = col[u] < p.nb;
-        if (SRC == T_MXFP4) {
-            const uint8_t *blk = (const uint8_t *)p.src + ((int64_t)row[u] * p.nb + (real ? col[u] : 0)) * 17;
-            raw[u][2] = blk[0];
-            __builtin_memcpy(&raw[u][0], blk + 1 + 8 * (a & 1), 8);
-            if (!real) raw[u][0] = raw[u][1] = raw[u][2] = 0;
-        } else {
-            mx_load8<SRC>(p.src, (int64_t)row[u] * p.ld + (real ? col[u] : 0) * 32 + 8 * a, v[u]);
-            if (!real) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
-            }
-        }
+        mx_source<SRC>(p, row[u], col[u], col[u] < p.nb, a, v[u], raw[u]);
     }
 #pragma unroll
     for (int u = 0; u < MX_U; ++u) {
         const bool in = b0 + 64 * u < p.nblk;
-        uint32_t codes = 0, e;
-        if (SRC == T_MXFP4) {
-            const int sh = 4 * (a >> 1);
-            codes = mx_gather((raw[u][0] >> sh) & 0x0f0f0f0fu) | (mx_gather((raw[u][1] >> sh) & 0x0f0f0f0fu) << 16);
-            e = raw[u][2];
-        } else {
-            float m = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[u][j]));      // (a NaN is passed over)
-            m = fmaxf(m, ffrom(mx_quad<0xB1>(fbits(m))));
-            m = fmaxf(m, ffrom(mx_quad<0x4E>(fbits(m))));
-            const int x = (int)(fbits(m) >> 23) - 2;
-            e = (uint32_t)(x < 0 ? 0 : x > 252 ? 252 : x);
-            const float inv = ffrom((254 - e) << 23);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) codes |= mx_code(v[u][j], inv) << (4 * j);
-        }
-        const bool real = col[u] < p.nb;
-        if (p.values && in && real)
-            *(uint4 *)(p.values + (int64_t)row[u] * p.ncol + col[u] * 32 + 8 * a) = mx_values(codes, e);
-        if (PACKED) {
-            const int64_t at = (int64_t)row[u] * p.row.d + col[u];
-            if (in) *(uint32_t *)(p.dst + at * 16 + 4 * a) = codes;
-            const uint32_t c = col[u];
-            if (in && a == 0) p.scales[(int64_t)row[u] * p.row.d + (c & ~15u) + 4 * (c & 3) + ((c >> 2) & 3)] = (uint8_t)e;
+        uint32_t e;
+        const uint32_t codes = mx_encode<SRC>(a, v[u], raw[u], e), c = col[u];
+        if (p.values && in && c < p.nb)
+            *(uint4 *)(p.values + (int64_t)row[u] * p.ncol + c * 32 + 8 * a) = mx_values(codes, e);
+        if (FORM == MX_ROWS) {
+            if (in) *(uint32_t *)(p.dst + ((int64_t)row[u] * p.row.d + c) * 16 + 4 * a) = codes;
+            if (in && a == 0)
+                p.scales[((int64_t)(c >> 4) * p.nrow + p.row0 + row[u]) * 16 + 4 * (c & 3) + ((c >> 2) & 3)] = (uint8_t)e;
         } else {
             // ggml's block: e, then byte j = value j | value j + 16 << 4; lane a gets bytes 4a .. 4a + 3
             const uint32_t lo = mx_quad<0x50>(codes) >> (16 * (a & 1)), hi = mx_quad<0xFA>(codes) >> (16 * (a & 1));
@@ -166,7 +182,7 @@ __global__ __launch_bounds__(256) void k_mx_quantize(MxQuantArgs p) {
             for (int j = 0; j < 4; ++j) o[1 + 4 * a + j] = (uint8_t)(w >> (8 * j));
         }
     }
-    if (!PACKED) {
+    if (FORM == MX_BLOCKS) {
         __syncthreads();
         const uint32_t first = blockIdx.x * (MX_U * 64);
         const uint32_t n = (p.nblk - first < MX_U * 64 ? p.nblk - first : MX_U * 64) * 17;
@@ -179,6 +195,37 @@ __global__ __launch_bounds__(256) void k_mx_quantize(MxQuantArgs p) {
             }
         }
     }
+}
+
+// tiles: a workgroup writes a strip's 512 columns, four pieces of 128; grid (np / 512, strips of the launch)
+template <int SRC>
+__global__ __launch_bounds__(256) void k_mx_tiles(MxQuantArgs p) {
+    __shared__ uint32_t es[64];
+    const int tid = threadIdx.x, a = tid & 3, q = (tid >> 2) & 3, r = tid >> 4;
+    const uint32_t strip = (uint32_t)p.row0 + blockIdx.y, mat = p.row.div(strip);
+    const int64_t in_mat = (int64_t)(strip - mat * p.row.d) * 16 + r, row = mat * p.nrow + in_mat;
+    float v[4][8];
+    uint32_t raw[4][3];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t col = blockIdx.x * 16 + 4 * c + q;
+        mx_source<SRC>(p, row, col, in_mat < p.nrow && col < p.nb, a, v[c], raw[c]);
+    }
+    uint8_t *d = p.dst + ((int64_t)strip * gridDim.x + blockIdx.x) * 4096;
+    uint32_t all = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t col = blockIdx.x * 16 + 4 * c + q;
+        uint32_t e;
+        const uint32_t codes = mx_encode<SRC>(a, v[c], raw[c], e);
+        all |= e << (8 * c);
+        *(uint32_t *)(d + c * 1024 + (16 * q + r) * 16 + 4 * a) = codes;
+        if (p.values && in_mat < p.nrow && col < p.nb)
+            *(uint4 *)(p.values + row * p.ncol + col * 32 + 8 * a) = mx_values(codes, e);
+    }
+    if (a == 0) es[16 * q + r] = all;
+    __syncthreads();
+    if (tid < 64) *(uint32_t *)(p.scales + ((int64_t)strip * gridDim.x + blockIdx.x) * 256 + 4 * tid) = es[tid];
 }
 
 // F32 / F16 rows as sums of BF16 rows: the top 16 bits, then those of the rest, which holds every bit of an F16 value

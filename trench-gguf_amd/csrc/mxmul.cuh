@@ -14,15 +14,15 @@
 typedef int mx_i8 __attribute__((ext_vector_type(8)));
 
 struct MxMulArgs {
-    const uint8_t *x;           // BF16 rows, or packed codes
-    const uint8_t *xs;          // packed scales
-    int64_t nx, xrow;           // rows of x and bytes from row to row (packed: of codes)
-    int64_t kx;                 // BF16: values of a row that are there (the rest of a 128 counts as zero)
-    int64_t piece;              // BF16: bytes from piece to piece
+    const uint8_t *x;           // BF16 rows (pieces of F16 and F32 rows one after the other), or codes (rows layout)
+    const uint8_t *xs;          // scales (rows layout)
+    int64_t nx, xrow;           // rows of x and bytes from row to row
+    int64_t kx;                 // BF16: values of a row that are there, its pieces together (the rest counts as zero)
     int pieces;
-    const uint8_t *w, *ws, *u, *us;     // packed weights and scales; u, us of the second product
-    int64_t nmat, ne1, np;      // np: padded row length
-    int nk;                     // 128-value pieces of a row
+    const uint8_t *w, *ws, *u, *us;     // codes and scales (tiles layout), u and us of the second product
+    int64_t nmat, ne1, strips;  // strips of 16 rows of a matrix
+    int nk;                     // 128-value pieces of a row of w that hold values
+    int nc;                     // 512-value pieces of a row of w (the last may be part padding)
     const int32_t *offsets, *rows;
     int64_t m;
     void *y;
@@ -119,9 +119,9 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
         }
         return;
     }
-    const int64_t wr = e * a.ne1 + (n0 + (lane & 15) < a.ne1 ? n0 + (lane & 15) : a.ne1 - 1);
-    const uint8_t *wp[2] = {a.w + wr * (a.np / 2) + 16 * q, GLU ? a.u + wr * (a.np / 2) + 16 * q : nullptr};
-    const uint8_t *sp[2] = {a.ws + wr * (a.np / 32) + 4 * q, GLU ? a.us + wr * (a.np / 32) + 4 * q : nullptr};
+    const int64_t strip = e * a.strips + blockIdx.x;
+    const uint8_t *wp[2] = {a.w + strip * a.nc * 4096 + 16 * lane, GLU ? a.u + strip * a.nc * 4096 + 16 * lane : nullptr};
+    const uint8_t *sp[2] = {a.ws + strip * a.nc * 256 + 4 * lane, GLU ? a.us + strip * a.nc * 256 + 4 * lane : nullptr};
     for (int64_t m0 = r0; m0 < r1; m0 += 16 * MF) {
         mx_f4 acc[MF][G];
         const uint8_t *xp[MF];
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
             const int64_t r = m0 + 16 * f + (lane & 15);
             const int64_t i = mx_row(a, r < r1 ? r : r1 - 1);
             xp[f] = a.x + (i < 0 ? 0 : i) * a.xrow;
-            xsp[f] = FP4 ? a.xs + (i < 0 ? 0 : i) * (a.np / 32) + 4 * q : nullptr;
+            xsp[f] = FP4 ? a.xs + (i < 0 ? 0 : i) * 16 + 4 * q : nullptr;
 #pragma unroll
             for (int g = 0; g < G; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
         }
@@ -141,36 +141,37 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
                 uint32_t sc[G];
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    wq[g] = *(const uint4 *)(wp[g] + (int64_t)c * 64);
-                    sc[g] = sp[g][(c >> 2) * 16 + (c & 3)];
+                    wq[g] = *(const uint4 *)(wp[g] + (int64_t)c * 1024);
+                    sc[g] = sp[g][(c >> 2) * 256 + (c & 3)];
                 }
                 if (FP4) {
 #pragma unroll
                     for (int f = 0; f < MF; ++f) {
                         const uint4 xq = *(const uint4 *)(xp[f] + (int64_t)c * 64 + 16 * q);
-                        const uint32_t xsc = xsp[f][(c >> 2) * 16 + (c & 3)];
+                        const uint32_t xsc = xsp[f][(c >> 2) * a.nx * 16 + (c & 3)];
 #pragma unroll
                         for (int g = 0; g < G; ++g)
                             acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
                                 mx_wide(wq[g]), mx_wide(xq), acc[f][g], 4, 4, 0, (int)sc[g], 0, (int)xsc);
                     }
                 } else {
-                    const bool in = c * 128 + 32 * q < a.kx;
+                    const int s = p * a.nk + c;
+                    const bool in = (int64_t)s * 128 + 32 * q < a.kx;
                     mx_bf8 xv[MF][4];
 #pragma unroll
                     for (int f = 0; f < MF; ++f) {
-                        const uint8_t *xc = xp[f] + p * a.piece + (int64_t)c * 256 + 64 * q;
+                        const uint8_t *xc = xp[f] + (int64_t)s * 256 + 64 * q;
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
                             xv[f][j] = *(const mx_bf8 *)(in ? xc + 16 * j : (const uint8_t *)mx_zero);
                     }
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        const float s = ffrom(sc[g] << 23);
+                        const float scale = ffrom(sc[g] << 23);
                         const uint32_t cw[4] = {wq[g].x, wq[g].y, wq[g].z, wq[g].w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const mx_bf8 wv = mx_widen(cw[j], s);
+                            const mx_bf8 wv = mx_widen(cw[j], scale);
 #pragma unroll
                             for (int f = 0; f < MF; ++f)
                                 acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[f][j], acc[f][g], 0, 0, 0);
@@ -258,26 +259,29 @@ DEV void mx_to_lds(const void *g, void *l) {       // 16 bytes a lane to l + 16 
     __builtin_amdgcn_global_load_lds((mx_gp)g, (mx_lp)l, 16, 0, 0);
 }
 
-// BF16 rows: WM x WN waves, each FM x 16 rows by FN x 16 columns (with GLU the first half of the FN are of w and the
-// second the same columns of u). x goes through LDS 128 values of k at a time, in two buffers; a row is 16 pieces of 16
-// bytes, piece 4q + c at (4c + q) ^ (row & 15), so that the reads of 16 rows spread over the banks. A wave's weights go
-// straight to its registers: as codes they are a quarter of what x takes.
-template <int WM, int WN, int FM, int FN, bool GLU>
+// WM x WN waves, each FM x 16 rows by FN x 16 columns (with GLU the first half of its FN strips are w's and the second
+// the same columns of u). x goes through LDS, 256 bytes of every row a step (128 BF16 values or 512 codes), in two
+// buffers: piece 4c + q of a row's 16, which lane group q takes into product c, lies at (4c + q) ^ (row & 15), so that
+// the reads of 16 rows spread over the banks. A wave's weights go straight to its registers, a kilobyte of a strip at a
+// time and one ahead: as codes they are a quarter of what BF16 rows take, and half of them are read twice.
+template <bool FP4, int WM, int WN, int FM, int FN, bool GLU>
 __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
-    constexpr int TM = WM * FM * 16, NO = WN * FN * 16 / (GLU ? 2 : 1), NW = WM * WN, LD = TM / 4 / NW;
+    constexpr int TM = WM * FM * 16, NS = WN * FN / (GLU ? 2 : 1), NO = NS * 16, NW = WM * WN, LD = TM / 4 / NW;
+    constexpr int FH = GLU ? FN / 2 : FN;                   // strips of one matrix
     __shared__ __align__(1024) uint8_t xs[2 * TM * 256];
-    const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, q = lane >> 4, wm = wave / WN, wn = wave % WN;
-    const int nt = (int)((a.ne1 + NO - 1) / NO), total = nt * a.mt, per = (total + 7) / 8;
+    __shared__ __align__(16) uint8_t xsc[FP4 ? 2 * TM * 16 : 16];
+    const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+    const int nt = (int)((a.strips + NS - 1) / NS), total = nt * a.mt, per = (total + 7) / 8;
     const int id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
     if ((int)(blockIdx.x / 8) >= per || id >= total) return;
     int64_t e, r0, r1;
     if (!mx_tile<TM>(a, id / nt, e, r0, r1)) return;
-    const int64_t nb = (int64_t)(id % nt) * NO + wn * (NO / WN);
+    const int64_t s0 = (int64_t)(id % nt) * NS;             // the tile's first strip
     if (e == a.nmat) {
-        const int64_t c0 = (int64_t)(id % nt) * NO;
         const float z[4] = {0.f, 0.f, 0.f, 0.f};
         for (int64_t i = tid; i < (r1 - r0) * (NO / 4); i += NW * 64) {
-            const int64_t n = c0 + 4 * (i % (NO / 4));
+            const int64_t n = s0 * 16 + 4 * (i % (NO / 4));
             if (n < a.ne1) mx_store4(a, r0 + i / (NO / 4), n, z);
         }
         return;
@@ -290,230 +294,122 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
         const int64_t r = r0 + row < r1 ? r0 + row : r1 - 1;
         const int64_t j = mx_row(a, r);
         const int p = (lane & 15) ^ (row & 15);
-        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * (4 * (p & 3) + (p >> 2));
+        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * (FP4 ? p : 4 * (p & 3) + (p >> 2));
     }
-    uint32_t wo[FN], so[FN];                // codes and scales of this lane's columns, from the tile's first
-    const int64_t n0 = e * a.ne1 + (int64_t)(id % nt) * NO;
-    const int nleft = (int)(a.ne1 - (int64_t)(id % nt) * NO);
-    const uint8_t *wb[2] = {a.w + n0 * (a.np / 2), GLU ? a.u + n0 * (a.np / 2) : nullptr};
-    const uint8_t *sb[2] = {a.ws + n0 * (a.np / 32), GLU ? a.us + n0 * (a.np / 32) : nullptr};
+    const uint8_t *sp = a.xs;               // FP4: a row's scales of 512 values, a lane each of the first TM
+    if (FP4) {
+        const int64_t r = r0 + tid < r1 ? r0 + tid : r1 - 1;
+        const int64_t j = mx_row(a, r);
+        sp += (j < 0 ? 0 : j) * 16;
+    }
+    const uint8_t *wp[FN], *wsp[FN];        // (uniform) this wave's strips, those past the last the last
 #pragma unroll
     for (int f = 0; f < FN; ++f) {
-        const int n = wn * (NO / WN) + (GLU ? f % (FN / 2) : f) * 16 + (lane & 15);
-        const uint32_t c = (uint32_t)(n < nleft ? n : nleft - 1);
-        wo[f] = c * (uint32_t)(a.np / 2) + 16 * q;
-        so[f] = c * (uint32_t)(a.np / 32) + 4 * q;
+        const int64_t t = s0 + wn * FH + f % FH, strip = e * a.strips + (t < a.strips ? t : a.strips - 1);
+        wp[f] = (f < FH ? a.w : a.u) + strip * a.nc * 4096;
+        wsp[f] = (f < FH ? a.ws : a.us) + strip * a.nc * 256;
     }
     mx_f4 acc[FN][FM];
 #pragma unroll
     for (int f = 0; f < FN; ++f)
 #pragma unroll
         for (int g = 0; g < FM; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
-    const int steps = a.nk * a.pieces;
-    // a row's pieces follow each other, so a step of x is always 256 bytes; those of the weights start over
-    auto stage = [&](int s, uint8_t *buf) {
-        if ((int64_t)s * 128 + 128 > a.kx) {        // (the last step, of rows that end inside it)
+    const int steps = FP4 ? a.nc : a.nk * a.pieces;
+    // part j of 4 of step s into its buffer
+    auto stage = [&](int s, int j) {
+        uint8_t *buf = xs + (s & 1) * (TM * 256);
+        if (!FP4 && (int64_t)s * 128 + 128 > a.kx) {        // (the last step, of rows that end inside it)
 #pragma unroll
-            for (int i = 0; i < LD; ++i) {
+            for (int i = j * LD / 4; i < (j + 1) * LD / 4; ++i) {
                 const int p = (lane & 15) ^ (((wave * LD + i) * 4 + (lane >> 4)) & 15);
                 const bool in = (int64_t)s * 128 + 8 * (4 * (p & 3) + (p >> 2)) < a.kx;
                 mx_to_lds(in ? xp[i] : (const uint8_t *)mx_zero, buf + (wave * LD + i) * 1024);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < LD; ++i) {
+            for (int i = j * LD / 4; i < (j + 1) * LD / 4; ++i) {
                 mx_to_lds(xp[i], buf + (wave * LD + i) * 1024);
                 xp[i] += 256;
             }
         }
+        if (FP4 && j == 3 && wave * 64 < TM) mx_to_lds(sp + (int64_t)s * a.nx * 16, xsc + (s & 1) * (TM * 16) + wave * 1024);
     };
-    uint4 wq[FN];
-    uint32_t sc[FN];
-    int c = 0;                              // the weights' next 128
-    auto fetch = [&]() {
+    uint4 wq[FN], wn_[FN];
+    uint32_t sc[FN], sn[FN];
+    auto fetch = [&](int c) {               // the weights' piece c
 #pragma unroll
-        for (int f = 0; f < FN; ++f) {
-            wq[f] = *(const uint4 *)(wb[GLU && f >= FN / 2] + (int64_t)c * 64 + wo[f]);
-            sc[f] = *(sb[GLU && f >= FN / 2] + ((c >> 2) * 16 + (c & 3)) + so[f]);
-        }
-        c = c + 1 < a.nk ? c + 1 : 0;
+        for (int f = 0; f < FN; ++f) wn_[f] = *(const uint4 *)(wp[f] + (int64_t)c * 1024 + 16 * lane);
     };
-    auto work = [&](const uint8_t *buf, const uint4 (&w)[FN], const uint32_t (&sv)[FN]) {
-        const uint8_t *b = buf + (wm * FM * 16 + (lane & 15)) * 256;
+    auto scales = [&](int c) {              // and the scales of its 512 values
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            mx_bf8 xv[FM], wv[FN];
-#pragma unroll
-            for (int g = 0; g < FM; ++g) xv[g] = *(const mx_bf8 *)(b + g * 4096 + (((4 * j + q) ^ (lane & 15)) * 16));
-#pragma unroll
-            for (int f = 0; f < FN; ++f)
-                wv[f] = mx_widen(j == 0 ? w[f].x : j == 1 ? w[f].y : j == 2 ? w[f].z : w[f].w, ffrom(sv[f] << 23));
-#pragma unroll
-            for (int g = 0; g < FM; ++g)
-#pragma unroll
-                for (int f = 0; f < FN; ++f)
-                    acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[f], xv[g], acc[f][g], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int f = 0; f < FN; ++f) sn[f] = *(const uint32_t *)(wsp[f] + (int64_t)c * 256 + 4 * lane);
     };
-    stage(0, xs);
-    fetch();
-    mx_sync();
-#pragma unroll 1
-    for (int s = 0; s < steps; ++s) {
-        uint4 w[FN];
-        uint32_t sv[FN];
+    int c = 0;                              // BF16: the piece at hand
 #pragma unroll
-        for (int f = 0; f < FN; ++f) {
-            w[f] = wq[f];
-            sv[f] = sc[f];
-        }
-        if (s + 1 < steps) {
-            stage(s + 1, xs + ((s + 1) & 1) * (TM * 256));
-            fetch();
-        }
-        work(xs + (s & 1) * (TM * 256), w, sv);
-        mx_sync();
-    }
-#pragma unroll
-    for (int g = 0; g < FM; ++g) {
-        const int64_t r = r0 + (wm * FM + g) * 16 + (lane & 15);
-        if (r >= r1) continue;
-        const bool on = mx_row(a, r) >= 0;
-#pragma unroll
-        for (int f = 0; f < (GLU ? FN / 2 : FN); ++f) {
-            const int64_t n = nb + f * 16 + 4 * q;
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = acc[f][g][i];
-                if (GLU) v[i] = mx_glu(v[i], acc[(f + FN / 2) % FN][g][i]);
-                if (!on) v[i] = 0.f;
-            }
-            if (n < a.ne1) mx_store4(a, r, n, v);
-        }
-    }
-}
-
-// Packed rows: both sides through LDS, 256 values of k (128 bytes a row) at a time in two buffers, the scales of 512
-// straight to registers. A row is 8 pieces of 16 bytes, piece p at p ^ (row / 2 & 7).
-template <int WM, int WN, int FM, int FN, bool GLU>
-__global__ __launch_bounds__(WM * WN * 64) void k_mx_tile4(MxMulArgs a) {
-    constexpr int TM = WM * FM * 16, TN = WN * FN * 16, NO = TN / (GLU ? 2 : 1), NW = WM * WN;
-    constexpr int LX = TM / 8 / NW, LW = TN / 8 / NW;
-    __shared__ __align__(1024) uint8_t buf[2 * (TM + TN) * 128];
-    const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, q = lane >> 4, wm = wave / WN, wn = wave % WN;
-    const int nt = (int)((a.ne1 + NO - 1) / NO), total = nt * a.mt, per = (total + 7) / 8;
-    const int id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    if ((int)(blockIdx.x / 8) >= per || id >= total) return;
-    int64_t e, r0, r1;
-    if (!mx_tile<TM>(a, id / nt, e, r0, r1)) return;
-    const int64_t nb = (int64_t)(id % nt) * NO;
-    if (e == a.nmat) {
-        const float z[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t i = tid; i < (r1 - r0) * (NO / 4); i += NW * 64) {
-            const int64_t n = nb + 4 * (i % (NO / 4));
-            if (n < a.ne1) mx_store4(a, r0 + i / (NO / 4), n, z);
-        }
-        return;
-    }
-    // tile row t of w: with GLU each wave's columns are half of w and half of u
-    auto wrow = [&](int t, bool &second) {
-        const int f = t / 16 % FN, v = t / (16 * FN);
-        second = GLU && f >= FN / 2;
-        const int64_t n = nb + v * (NO / WN) + (GLU ? f % (FN / 2) : f) * 16 + t % 16;
-        return e * a.ne1 + (n < a.ne1 ? n : a.ne1 - 1);
-    };
-    const uint8_t *xp[LX], *wp[LW];
-#pragma unroll
-    for (int i = 0; i < LX; ++i) {
-        const int row = (wave * LX + i) * 8 + (lane >> 3);
-        const int64_t r = r0 + row < r1 ? r0 + row : r1 - 1;
-        const int64_t j = mx_row(a, r);
-        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * ((lane & 7) ^ ((row >> 1) & 7));
-    }
-#pragma unroll
-    for (int i = 0; i < LW; ++i) {
-        const int row = (wave * LW + i) * 8 + (lane >> 3);
-        bool second;
-        const int64_t n = wrow(row, second);
-        wp[i] = (second ? a.u : a.w) + n * (a.np / 2) + 16 * ((lane & 7) ^ ((row >> 1) & 7));
-    }
-    const uint8_t *xsp[FM], *wsp[FN];
-#pragma unroll
-    for (int g = 0; g < FM; ++g) {
-        const int row = (wm * FM + g) * 16 + (lane & 15);
-        const int64_t r = r0 + row < r1 ? r0 + row : r1 - 1;
-        const int64_t j = mx_row(a, r);
-        xsp[g] = a.xs + (j < 0 ? 0 : j) * (a.np / 32) + 4 * q;
-    }
-#pragma unroll
-    for (int f = 0; f < FN; ++f) {
-        bool second;
-        const int64_t n = wrow((wn * FN + f) * 16 + (lane & 15), second);
-        wsp[f] = (second ? a.us : a.ws) + n * (a.np / 32) + 4 * q;
-    }
-    mx_f4 acc[FN][FM];
-#pragma unroll
-    for (int f = 0; f < FN; ++f)
-#pragma unroll
-        for (int g = 0; g < FM; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
-    auto stage = [&](uint8_t *buf) {
-#pragma unroll
-        for (int i = 0; i < LX; ++i) {
-            mx_to_lds(xp[i], buf + (wave * LX + i) * 1024);
-            xp[i] += 128;
-        }
-#pragma unroll
-        for (int i = 0; i < LW; ++i) {
-            mx_to_lds(wp[i], buf + TM * 128 + (wave * LW + i) * 1024);
-            wp[i] += 128;
-        }
-    };
-    uint32_t xc[FM], wc[FN], xn[FM], wn_[FN];
-    auto scales = [&](int c) {
-#pragma unroll
-        for (int g = 0; g < FM; ++g) xn[g] = *(const uint32_t *)(xsp[g] + (int64_t)c * 16);
-#pragma unroll
-        for (int f = 0; f < FN; ++f) wn_[f] = *(const uint32_t *)(wsp[f] + (int64_t)c * 16);
-    };
-    const int sw = (lane >> 1) & 7;
-    auto work = [&](const uint8_t *buf) {
-        const uint8_t *x = buf + (wm * FM * 16 + (lane & 15)) * 128, *w = buf + (TM + wn * FN * 16 + (lane & 15)) * 128;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint4 xv[FM], wv[FN];
-#pragma unroll
-            for (int f = 0; f < FN; ++f) wv[f] = *(const uint4 *)(w + f * 2048 + ((4 * h + q) ^ sw) * 16);
-#pragma unroll
-            for (int g = 0; g < FM; ++g) xv[g] = *(const uint4 *)(x + g * 2048 + ((4 * h + q) ^ sw) * 16);
-#pragma unroll
-            for (int g = 0; g < FM; ++g)
-#pragma unroll
-                for (int f = 0; f < FN; ++f)
-                    acc[f][g] = h == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                             mx_wide(wv[f]), mx_wide(xv[g]), acc[f][g], 4, 4, 0, (int)wc[f], 0, (int)xc[g])
-                                       : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                             mx_wide(wv[f]), mx_wide(xv[g]), acc[f][g], 4, 4, 1, (int)wc[f], 1, (int)xc[g]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    const int steps = (a.nk + 1) / 2;
-    stage(buf);
+    for (int j = 0; j < 4; ++j) stage(0, j);
+    fetch(0);
     scales(0);
     mx_sync();
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
-        // the scales of two steps come as one dword a row
+        const uint8_t *b = xs + (s & 1) * (TM * 256) + (wm * FM * 16 + (lane & 15)) * 256;
+        const bool more = s + 1 < steps;
+        uint32_t xc[FP4 ? FM : 1];
+        const int next = FP4 ? s + 1 : c + 1 < a.nk ? c + 1 : 0;
+        if (FP4) {
 #pragma unroll
-        for (int g = 0; g < FM; ++g) xc[g] = s & 1 ? xn[g] >> 16 : xn[g];
+            for (int g = 0; g < FM; ++g)
+                xc[g] = *(const uint32_t *)(xsc + (s & 1) * (TM * 16) + ((wm * FM + g) * 16 + (lane & 15)) * 16 + 4 * q);
 #pragma unroll
-        for (int f = 0; f < FN; ++f) wc[f] = s & 1 ? wn_[f] >> 16 : wn_[f];
-        if (s + 1 < steps) {
-            stage(buf + ((s + 1) & 1) * ((TM + TN) * 128));
-            if (s & 1) scales((s + 1) >> 1);
+            for (int f = 0; f < FN; ++f) sc[f] = sn[f];
+            if (more) scales(next);
+        } else {
+#pragma unroll
+            for (int f = 0; f < FN; ++f) {
+                wq[f] = wn_[f];
+                sc[f] = ((sn[f] >> (8 * (c & 3))) & 255) << 23;
+            }
+            if (more) {
+                fetch(next);
+                if ((next & 3) == 0) scales(next >> 2);
+            }
         }
-        work(buf + (s & 1) * ((TM + TN) * 128));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (FP4) {
+                if (4 * s + j >= a.nk) continue;            // (padding)
+#pragma unroll
+                for (int f = 0; f < FN; ++f) wq[f] = wn_[f];
+                if (j < 3 || more) fetch(4 * s + j + 1);    // (the last piece of a row is followed by its scales at least)
+            }
+            if (more) stage(s + 1, j);
+            mx_bf8 wv[FN];
+            if (!FP4) {
+#pragma unroll
+                for (int f = 0; f < FN; ++f)
+                    wv[f] = mx_widen(j == 0 ? wq[f].x : j == 1 ? wq[f].y : j == 2 ? wq[f].z : wq[f].w, ffrom(sc[f]));
+            }
+#pragma unroll
+            for (int g = 0; g < FM; ++g) {
+                const uint4 xv = *(const uint4 *)(b + g * 4096 + (((4 * j + q) ^ (lane & 15)) * 16));
+                union { uint4 u; mx_bf8 b; } xb = {xv};
+#pragma unroll
+                for (int f = 0; f < FN; ++f) {
+                    if (FP4) {
+                        const mx_i8 wi = mx_wide(wq[f]), xi = mx_wide(xv);
+                        const int ws = (int)sc[f], xw = (int)xc[FP4 ? g : 0];
+                        acc[f][g] = j == 0   ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wi, xi, acc[f][g], 4, 4, 0, ws, 0, xw)
+                                    : j == 1 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wi, xi, acc[f][g], 4, 4, 1, ws, 1, xw)
+                                    : j == 2 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wi, xi, acc[f][g], 4, 4, 2, ws, 2, xw)
+                                             : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wi, xi, acc[f][g], 4, 4, 3, ws, 3, xw);
+                    } else {
+                        acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[f], xb.b, acc[f][g], 0, 0, 0);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (!FP4) c = next;
         mx_sync();
     }
 #pragma unroll
@@ -522,13 +418,13 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile4(MxMulArgs a) {
         if (r >= r1) continue;
         const bool on = mx_row(a, r) >= 0;
 #pragma unroll
-        for (int f = 0; f < (GLU ? FN / 2 : FN); ++f) {
-            const int64_t n = nb + wn * (NO / WN) + f * 16 + 4 * q;
+        for (int f = 0; f < FH; ++f) {
+            const int64_t n = (s0 + wn * FH + f) * 16 + 4 * q;
             float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 v[i] = acc[f][g][i];
-                if (GLU) v[i] = mx_glu(v[i], acc[(f + FN / 2) % FN][g][i]);
+                if (GLU) v[i] = mx_glu(v[i], acc[(f + FH) % FN][g][i]);
                 if (!on) v[i] = 0.f;
             }
             if (n < a.ne1) mx_store4(a, r, n, v);

@@ -15,8 +15,12 @@ from gpuq import BF16, F16, F32, MXFP4
 
 TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
-# a packed MXFP4 tensor on the device: the bytes and [nmat, ne1, ne0] (rows: nmat 1)
+BLOCKS, ROWS, TILES = 0, 1, 2           # the forms of MXFP4 data (include/gpuq.h)
+
+# stored MXFP4 matrices laid out for products: the bytes (tiles) and [nmat, ne1, ne0]
 Packed = namedtuple("Packed", "data nmat ne1 ne0")
+# MXFP4 rows to multiply: the bytes (rows) and [n, ncol]
+Rows = namedtuple("Rows", "data n ncol")
 # assignments sorted by expert: offsets [nexp + 1], the token of each place and its index among the ids, all int32
 Group = namedtuple("Group", "offsets rows slots")
 
@@ -37,39 +41,50 @@ def _rows(x):
 
 def pack(gq, blocks, nmat, ne1, ne0):
     """ggml's MXFP4 blocks (uint8 on the device, nmat x ne1 rows of ne0 values) -> Packed, bit for bit"""
-    if blocks.dtype != torch.uint8 or not blocks.is_contiguous() or ne0 % 32 or \
-            blocks.numel() != nmat * ne1 * (ne0 // 32) * 17:
-        raise ValueError("expected %d contiguous bytes of MXFP4 blocks" % (nmat * ne1 * (ne0 // 32) * 17))
-    size = gq.gpuq_mxfp4_packed_bytes(nmat * ne1, ne0)
+    size = gq.gpuq_mxfp4_bytes(TILES, nmat, ne1, ne0)
+    want = gq.gpuq_mxfp4_bytes(BLOCKS, nmat, ne1, ne0)
+    if not size or blocks.dtype != torch.uint8 or not blocks.is_cuda or not blocks.is_contiguous() or \
+            blocks.numel() != want:
+        raise ValueError("expected %d contiguous bytes of MXFP4 blocks on the GPU" % want)
     out = torch.empty(size, dtype=torch.uint8, device=blocks.device)
-    if not size or gq.gpuq_mxfp4_quantize_dev(MXFP4, blocks.data_ptr(), nmat * ne1, ne0, ne0, 1, out.data_ptr(), None,
-                                              _stream(blocks)) != size:
+    if gq.gpuq_mxfp4_quantize_dev(MXFP4, blocks.data_ptr(), nmat, ne1, ne0, ne0, TILES, out.data_ptr(), None,
+                                  _stream(blocks)) != size:
         raise ValueError("gpuq_mxfp4_quantize_dev refused %d x %d x %d blocks" % (nmat, ne1, ne0))
     return Packed(out, nmat, ne1, ne0)
 
 
-def _quantize(gq, x, packed, values):
+def _quantize(gq, x, nmat, form, values):
     typ, ptr, n, ncol, ld = _rows(x)
-    size = gq.gpuq_mxfp4_packed_bytes(n, ncol) if packed else n * (ncol // 32) * 17
+    size = gq.gpuq_mxfp4_bytes(form, nmat, n // nmat, ncol)
     out = torch.empty(size, dtype=torch.uint8, device=x.device)
     back = torch.empty((n, ncol), dtype=torch.bfloat16, device=x.device) if values else None
-    got = gq.gpuq_mxfp4_quantize_dev(typ, ptr, n, ncol, ld, int(packed), out.data_ptr(),
-                                     back.data_ptr() if values else None, _stream(x)) if size else 0
-    if not got or got != size:
+    if not size or gq.gpuq_mxfp4_quantize_dev(typ, ptr, nmat, n // nmat, ncol, ld, form, out.data_ptr(),
+                                              back.data_ptr() if values else None, _stream(x)) != size:
         raise ValueError("gpuq_mxfp4_quantize_dev refused %d x %d (rows of whole 32s, 16-byte aligned)" % (n, ncol))
     return out, back
 
 
 def quantize(gq, x, values=False):
-    """rows rounded to MXFP4, Packed; with values also what they stand for, BF16 [n, ncol]: (Packed, values)"""
-    out, back = _quantize(gq, x, True, values)
-    p = Packed(out, 1, x.shape[0], x.shape[1])
-    return (p, back) if values else p
+    """rows rounded to MXFP4 to multiply: Rows; with values also what they stand for, BF16 [n, ncol]: (Rows, values)"""
+    out, back = _quantize(gq, x, 1, ROWS, values)
+    r = Rows(out, x.shape[0], x.shape[1])
+    return (r, back) if values else r
+
+
+def quantize_weights(gq, w, values=False):
+    """matrices [nmat, ne1, ne0] (or one, [ne1, ne0]) rounded to MXFP4 to multiply with: Packed; with values
+    (Packed, BF16 [nmat, ne1, ne0])"""
+    w = w if w.dim() == 3 else w[None]
+    if not w.is_contiguous():
+        raise ValueError("matrices must be contiguous")
+    out, back = _quantize(gq, w.view(-1, w.shape[2]), w.shape[0], TILES, values)
+    p = Packed(out, *w.shape)
+    return (p, back.view(w.shape)) if values else p
 
 
 def quantize_blocks(gq, x, values=False):
     """rows rounded to MXFP4 as ggml's blocks, uint8 [n, ncol / 32 * 17]; with values (blocks, values)"""
-    out, back = _quantize(gq, x, False, values)
+    out, back = _quantize(gq, x, 1, BLOCKS, values)
     out = out.view(x.shape[0], -1)
     return (out, back) if values else out
 
@@ -81,12 +96,12 @@ def _index(t, name):
 
 
 def matmul(gq, x, w, group=None, up=None, out_dtype=torch.float32):
-    """x [n, ne0] (F32, F16, BF16 or Packed rows) times w (Packed [nmat, ne1, ne0]) transposed -> [m, ne1].
+    """x [n, ne0] (F32, F16, BF16 or Rows) times w (Packed [nmat, ne1, ne0]) transposed -> [m, ne1].
 
     Without a group m = n and w is one matrix; with one (Group, from `group`) output row r is x[group.rows[r]] times the
     matrix whose offsets hold r, zero where none does. up: a second Packed like w, for silu(x w^T) * (x up^T)."""
-    if isinstance(x, Packed):
-        typ, ptr, n, ncol, ld, dev = MXFP4, x.data.data_ptr(), x.nmat * x.ne1, x.ne0, x.ne0, x.data.device
+    if isinstance(x, Rows):
+        typ, ptr, n, ncol, ld, dev = MXFP4, x.data.data_ptr(), x.n, x.ncol, x.ncol, x.data.device
     else:
         typ, ptr, n, ncol, ld = _rows(x)
         dev = x.device
