@@ -248,15 +248,19 @@ template <int TM> DEV bool mx_tile(const MxMulArgs &a, int t, int64_t &e, int64_
     return false;
 }
 
-typedef const __attribute__((address_space(1))) void *mx_gp;
-typedef __attribute__((address_space(3))) void *mx_lp;
+// 16 bytes a lane from g to l + 16 * lane (l the same in the wave), without registers between. Written out because the
+// compiler lets every later read of LDS wait for the builtin's loads, which are for the buffer that is not being read:
+// products then wait for the loads of the next step in every step. It names no register that the load writes; mx_sync
+// waits for it. (The wait states are those of reading m0 after a scalar write.)
+DEV void mx_to_lds(const void *g, void *l) {
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)l;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(g) : "memory");
+}
 // the loads into LDS have landed, for every wave
 DEV void mx_sync() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-}
-DEV void mx_to_lds(const void *g, void *l) {       // 16 bytes a lane to l + 16 * lane (l uniform)
-    __builtin_amdgcn_global_load_lds((mx_gp)g, (mx_lp)l, 16, 0, 0);
 }
 
 // WM x WN waves, each FM x 16 rows by FN x 16 columns (with GLU the first half of its FN strips are w's and the second
