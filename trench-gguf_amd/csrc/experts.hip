@@ -36,35 +36,41 @@ template <int SRC> void launch_quantize(int form, const MxQuantArgs &p, hipStrea
 int pieces_of(int x_type) { return x_type == T_F32 ? 3 : x_type == T_F16 ? 2 : 1; }
 int64_t round128(int64_t n) { return (n + 127) / 128 * 128; }
 
-template <int MF> void launch_rows(bool fp4, bool glu, const MxMulArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)a.strips, (unsigned)(a.offsets ? a.nmat + 1 : 1));
-#define MX_ROWS(F, G) hipLaunchKernelGGL((k_mx_rows<F, MF, G>), grid, dim3(512), 0, st, a)
+template <int MF, int NF> void launch_rows(bool fp4, bool glu, const MxMulArgs &a, hipStream_t st) {
+    const dim3 grid((unsigned)((a.strips + NF - 1) / NF), (unsigned)(a.offsets ? std::min(a.nmat, a.m) + 1 : 1));
+#define MX_ROWS_K(F, G) hipLaunchKernelGGL((k_mx_rows<F, MF, NF, G>), grid, dim3(512), 0, st, a)
     if (fp4) {
-        if (glu) MX_ROWS(true, true);
-        else MX_ROWS(true, false);
+        if (glu) MX_ROWS_K(true, true);
+        else MX_ROWS_K(true, false);
     } else {
-        if (glu) MX_ROWS(false, true);
-        else MX_ROWS(false, false);
+        if (glu) MX_ROWS_K(false, true);
+        else MX_ROWS_K(false, false);
     }
-#undef MX_ROWS
+#undef MX_ROWS_K
 }
 
-template <int WM, int WN, int FM, int FN> bool launch_tile(bool fp4, bool glu, MxMulArgs &a, hipStream_t st) {
-    constexpr int TM = WM * FM * 16, TN = WN * FN * 16;
-    const int64_t no = glu ? TN / 2 : TN, nt = (a.ne1 + no - 1) / no;
+// the row tiles of the grid and its workgroups, 0 for too many
+template <int TM, int TN> int64_t tile_grid(bool glu, MxMulArgs &a) {
+    const int64_t ns = TN / 16 / (glu ? 2 : 1), nt = (a.strips + ns - 1) / ns;
     const int64_t mt = (a.m + TM - 1) / TM + (a.offsets ? a.nmat + 1 : 0);
-    if (nt * mt >= ((int64_t)1 << 30)) return false;
+    if (nt * mt >= ((int64_t)1 << 30)) return 0;
     a.mt = (int)mt;
-    const dim3 grid((unsigned)((nt * mt + 7) / 8 * 8)), block(WM * WN * 64);
-#define MX_TILE(F, G) hipLaunchKernelGGL((k_mx_tile<F, WM, WN, FM, FN, G>), grid, block, 0, st, a)
-    if (fp4) {
-        if (glu) MX_TILE(true, true);
-        else MX_TILE(true, false);
-    } else {
-        if (glu) MX_TILE(false, true);
-        else MX_TILE(false, false);
-    }
-#undef MX_TILE
+    return (nt * mt + 7) / 8 * 8;
+}
+
+template <int WN, int FM, int FN> bool launch_tile(bool glu, MxMulArgs &a, hipStream_t st) {
+    const int64_t grid = tile_grid<FM * 16, WN * FN * 16>(glu, a);
+    if (!grid) return false;
+    if (glu) hipLaunchKernelGGL((k_mx_tile<WN, FM, FN, true>), dim3((unsigned)grid), dim3(WN * 64), 0, st, a);
+    else hipLaunchKernelGGL((k_mx_tile<WN, FM, FN, false>), dim3((unsigned)grid), dim3(WN * 64), 0, st, a);
+    return true;
+}
+
+template <int WM, int WN, int FM, int FN> bool launch_tile4(bool glu, MxMulArgs &a, hipStream_t st) {
+    const int64_t grid = tile_grid<WM * FM * 16, WN * FN * 16>(glu, a);
+    if (!grid) return false;
+    if (glu) hipLaunchKernelGGL((k_mx_tile4<WM, WN, FM, FN, true>), dim3((unsigned)grid), dim3(WM * WN * 64), 0, st, a);
+    else hipLaunchKernelGGL((k_mx_tile4<WM, WN, FM, FN, false>), dim3((unsigned)grid), dim3(WM * WN * 64), 0, st, a);
     return true;
 }
 
@@ -207,11 +213,12 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
     }
     const bool glu = d_up != nullptr;
     const int64_t per = m / nmat;                               // rows a group, on average
-    if (per <= 16) launch_rows<1>(fp4, glu, a, st);
-    else if (per <= 64) launch_rows<4>(fp4, glu, a, st);
-    else if (per < 256) {
-        if (!launch_tile<2, 2, 4, 4>(fp4, glu, a, st)) return 0;
-    } else if (!launch_tile<2, 4, 8, 4>(fp4, glu, a, st)) {
+    const int64_t tiles = (m + 127) / 128 * ((strips * (glu ? 2 : 1) + 15) / 16);       // 128 x 256
+    if (per <= 16) launch_rows<1, 1>(fp4, glu, a, st);
+    else if (per <= 64) launch_rows<4, 1>(fp4, glu, a, st);
+    else if (fp4) {
+        if (per < 256 ? !launch_tile4<2, 4, 4, 2>(glu, a, st) : !launch_tile4<2, 4, 8, 4>(glu, a, st)) return 0;
+    } else if (tiles < 1024 ? !launch_tile<4, 4, 4>(glu, a, st) : !launch_tile<4, 8, 4>(glu, a, st)) {
         return 0;
     }
     return hipGetLastError() == hipSuccess ? (size_t)(m * ne1 * type_size(y_type)) : 0;

@@ -102,82 +102,146 @@ DEV mx_bf8 mx_widen(uint32_t codes, float s) {
 
 DEV mx_i8 mx_wide(uint4 v) { return mx_i8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
 
-// ---- few rows a group: a workgroup owns 16 columns of one group, its 8 waves split k by 128-value pieces and their
-// sums meet in LDS in a fixed order; MF x 16 rows at a time. grid (ceil(ne1 / 16), groups + 1)
-template <bool FP4, int MF, bool GLU>
-__global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
-    constexpr int G = GLU ? 2 : 1;
-    __shared__ mx_f4 red[8][MF * G][64];
-    const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, q = lane >> 4;
-    const int64_t e = blockIdx.y, n0 = (int64_t)blockIdx.x * 16;
-    int64_t r0, r1;
-    mx_group(a, e, r0, r1);
-    if (e == a.nmat) {          // rows that belong to no expert
-        for (int64_t i = r0 * 4 + tid; i < r1 * 4; i += 512) {
-            const float z[4] = {0.f, 0.f, 0.f, 0.f};
-            if (n0 + 4 * (i & 3) < a.ne1) mx_store4(a, i >> 2, n0 + 4 * (i & 3), z);
+// rows that no group has: zeros, in NO columns from n0 on
+template <int NO> DEV void mx_clear(const MxMulArgs &a, int64_t r0, int64_t r1, int64_t n0, int threads) {
+    const float z[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t i = threadIdx.x; i < (r1 - r0) * (NO / 4); i += threads) {
+        const int64_t n = n0 + 4 * (i % (NO / 4));
+        if (n < a.ne1) mx_store4(a, r0 + i / (NO / 4), n, z);
+    }
+}
+
+// a lane's part of an address, opaque so that it stays a 32-bit offset beside a scalar address: the compiler would keep
+// the sum of both, a pair of registers for every strip
+DEV uint32_t mx_opaque(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// ---- few rows a group: a workgroup owns NF strips of one group, its 8 waves split k by 128-value pieces and their sums
+// meet in LDS in a fixed order; MF x 16 rows at a time. The weights' bytes bound it, so each wave keeps the loads of two
+// pieces ahead of its products in flight. grid (ceil(strips / NF), groups that can have rows + 1)
+
+// the y-th group that has rows (the last workgroup row: the rows of no group); false where there is none
+DEV bool mx_group_at(const MxMulArgs &a, int y, int64_t &e, int64_t &r0, int64_t &r1) {
+    if (!a.offsets) {
+        e = 0;
+        r0 = 0;
+        r1 = a.m;
+        return true;
+    }
+    if (y + 1 == (int)gridDim.y) {
+        e = a.nmat;
+        mx_group(a, e, r0, r1);
+        return r0 < r1;
+    }
+    const int lane = lane_id();
+    for (int64_t g0 = 0; g0 < a.nmat; g0 += 64) {
+        int64_t s0 = 0, s1 = 0;
+        if (g0 + lane < a.nmat) mx_group(a, g0 + lane, s0, s1);
+        uint64_t some = __ballot(s0 < s1);
+        const int n = __popcll(some);
+        if (y < n) {
+            for (; y > 0; --y) some &= some - 1;
+            const int l = __ffsll((unsigned long long)some) - 1;
+            e = g0 + l;
+            r0 = __builtin_amdgcn_readlane((int)s0, l);
+            r1 = __builtin_amdgcn_readlane((int)s1, l);
+            return true;
         }
+        y -= n;
+    }
+    return false;
+}
+
+template <bool FP4, int MF, int NF, bool GLU>
+__global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
+    constexpr int G = NF * (GLU ? 2 : 1), D = MF == 1 ? 3 : 2;      // streams of weights; pieces in flight
+    __shared__ mx_f4 red[8][MF * G][64];
+    const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t s0 = (int64_t)blockIdx.x * NF;
+    int64_t e, r0, r1;
+    if (!mx_group_at(a, (int)blockIdx.y, e, r0, r1)) return;
+    if (e == a.nmat) {
+        mx_clear<NF * 16>(a, r0, r1, s0 * 16, 512);
         return;
     }
-    const int64_t strip = e * a.strips + blockIdx.x;
-    const uint8_t *wp[2] = {a.w + strip * a.nc * 4096 + 16 * lane, GLU ? a.u + strip * a.nc * 4096 + 16 * lane : nullptr};
-    const uint8_t *sp[2] = {a.ws + strip * a.nc * 256 + 4 * lane, GLU ? a.us + strip * a.nc * 256 + 4 * lane : nullptr};
+    const uint8_t *wp[G], *sp[G];           // (uniform) strips past the last are the last
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const int64_t strip = e * a.strips + (s0 + g % NF < a.strips ? s0 + g % NF : a.strips - 1);
+        wp[g] = (g < NF ? a.w : a.u) + strip * a.nc * 4096;
+        sp[g] = (g < NF ? a.ws : a.us) + strip * a.nc * 256;
+    }
+    const int total = FP4 ? a.nk : a.nk * a.pieces;
     for (int64_t m0 = r0; m0 < r1; m0 += 16 * MF) {
         mx_f4 acc[MF][G];
-        const uint8_t *xp[MF];
-        const uint8_t *xsp[MF];
+        const uint8_t *xp[MF], *xsp[MF];
 #pragma unroll
         for (int f = 0; f < MF; ++f) {
             const int64_t r = m0 + 16 * f + (lane & 15);
             const int64_t i = mx_row(a, r < r1 ? r : r1 - 1);
-            xp[f] = a.x + (i < 0 ? 0 : i) * a.xrow;
+            xp[f] = a.x + (i < 0 ? 0 : i) * a.xrow + (FP4 ? 16 : 64) * q;
             xsp[f] = FP4 ? a.xs + (i < 0 ? 0 : i) * 16 + 4 * q : nullptr;
 #pragma unroll
             for (int g = 0; g < G; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
         }
-        for (int p = 0; p < a.pieces; ++p) {
-            for (int c = wave; c < a.nk; c += 8) {
-                uint4 wq[G];
-                uint32_t sc[G];
+        uint4 wq[D][G], xv[D][MF][FP4 ? 1 : 4];
+        uint32_t sc[D][G], xc[D][MF];
+        auto load = [&](int s, int d) {     // piece s
+            const int c = FP4 ? s : s % a.nk;
+            const uint32_t at = mx_opaque(16u * (uint32_t)lane);
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    wq[g] = *(const uint4 *)(wp[g] + (int64_t)c * 1024);
-                    sc[g] = sp[g][(c >> 2) * 256 + (c & 3)];
+            for (int g = 0; g < G; ++g) {
+                wq[d][g] = *(const uint4 *)(wp[g] + (int64_t)c * 1024 + at);
+                sc[d][g] = *(sp[g] + (int64_t)(c >> 2) * 256 + ((c & 3) + (at >> 2)));
+            }
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+                if (FP4) {
+                    xv[d][f][0] = *(const uint4 *)(xp[f] + (int64_t)c * 64);
+                    xc[d][f] = xsp[f][(int64_t)(c >> 2) * a.nx * 16 + (c & 3)];
+                } else {
+                    const bool in = (int64_t)s * 128 + 32 * q < a.kx;
+#pragma unroll
+                    for (int j = 0; j < (FP4 ? 1 : 4); ++j)
+                        xv[d][f][j] = *(const uint4 *)(in ? xp[f] + (int64_t)s * 256 + 16 * j : (const uint8_t *)mx_zero);
                 }
+            }
+        };
+        auto work = [&](int d) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
                 if (FP4) {
 #pragma unroll
-                    for (int f = 0; f < MF; ++f) {
-                        const uint4 xq = *(const uint4 *)(xp[f] + (int64_t)c * 64 + 16 * q);
-                        const uint32_t xsc = xsp[f][(c >> 2) * a.nx * 16 + (c & 3)];
-#pragma unroll
-                        for (int g = 0; g < G; ++g)
-                            acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                mx_wide(wq[g]), mx_wide(xq), acc[f][g], 4, 4, 0, (int)sc[g], 0, (int)xsc);
-                    }
+                    for (int f = 0; f < MF; ++f)
+                        acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                            mx_wide(wq[d][g]), mx_wide(xv[d][f][0]), acc[f][g], 4, 4, 0, (int)sc[d][g], 0, (int)xc[d][f]);
                 } else {
-                    const int s = p * a.nk + c;
-                    const bool in = (int64_t)s * 128 + 32 * q < a.kx;
-                    mx_bf8 xv[MF][4];
+                    const float scale = ffrom(sc[d][g] << 23);
+                    const uint32_t cw[4] = {wq[d][g].x, wq[d][g].y, wq[d][g].z, wq[d][g].w};
 #pragma unroll
-                    for (int f = 0; f < MF; ++f) {
-                        const uint8_t *xc = xp[f] + (int64_t)s * 256 + 64 * q;
+                    for (int j = 0; j < (FP4 ? 1 : 4); ++j) {
+                        const mx_bf8 wv = mx_widen(cw[j], scale);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            xv[f][j] = *(const mx_bf8 *)(in ? xc + 16 * j : (const uint8_t *)mx_zero);
-                    }
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const float scale = ffrom(sc[g] << 23);
-                        const uint32_t cw[4] = {wq[g].x, wq[g].y, wq[g].z, wq[g].w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const mx_bf8 wv = mx_widen(cw[j], scale);
-#pragma unroll
-                            for (int f = 0; f < MF; ++f)
-                                acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[f][j], acc[f][g], 0, 0, 0);
+                        for (int f = 0; f < MF; ++f) {
+                            union { uint4 u; mx_bf8 b; } x = {xv[d][f][j]};
+                            acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, x.b, acc[f][g], 0, 0, 0);
                         }
                     }
                 }
+            }
+        };
+        // (a load past the end is of the last piece and not used)
+#pragma unroll
+        for (int d = 0; d < D - 1; ++d) load(wave + 8 * d < total ? wave + 8 * d : total - 1, d);
+        for (int s = wave; s < total; s += 8 * D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                const int ahead = s + 8 * (d + D - 1);
+                load(ahead < total ? ahead : total - 1, (d + D - 1) % D);
+                if (s + 8 * d < total) work(d);
             }
         }
 #pragma unroll
@@ -185,23 +249,24 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
 #pragma unroll
             for (int g = 0; g < G; ++g) red[wave][f * G + g][lane] = acc[f][g];
         __syncthreads();
-        for (int f = wave; f < MF; f += 8) {
-            float v[G][4];
+        for (int i = wave; i < MF * NF; i += 8) {           // fragment f of strip k
+            const int f = i / NF, k = i % NF;
+            float v[2][4];
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                mx_f4 s = red[0][f * G + g][lane];
+            for (int h = 0; h < (GLU ? 2 : 1); ++h) {
+                mx_f4 sum = red[0][f * G + h * NF + k][lane];
 #pragma unroll
-                for (int w = 1; w < 8; ++w) s += red[w][f * G + g][lane];
+                for (int w = 1; w < 8; ++w) sum += red[w][f * G + h * NF + k][lane];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[g][i] = s[i];
+                for (int j = 0; j < 4; ++j) v[h][j] = sum[j];
             }
-            const int64_t r = m0 + 16 * f + (lane & 15), n = n0 + 4 * q;
+            const int64_t r = m0 + 16 * f + (lane & 15), n = (s0 + k) * 16 + 4 * q;
             if (r < r1 && n < a.ne1) {
                 const bool on = mx_row(a, r) >= 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (GLU) v[0][i] = mx_glu(v[0][i], v[G - 1][i]);
-                    if (!on) v[0][i] = 0.f;
+                for (int j = 0; j < 4; ++j) {
+                    if (GLU) v[0][j] = mx_glu(v[0][j], v[GLU ? 1 : 0][j]);
+                    if (!on) v[0][j] = 0.f;
                 }
                 mx_store4(a, r, n, v[0]);
             }
@@ -212,16 +277,35 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
 
 // ---- many rows: tiles of TM rows by TN columns
 
-// the row tile t of the grid: its group and rows. Groups take ceil(rows / TM) tiles each, in order, the rows of no
-// expert last. False for a tile past the last.
-template <int TM> DEV bool mx_tile(const MxMulArgs &a, int t, int64_t &e, int64_t &r0, int64_t &r1) {
+// The tile of this workgroup: its group, rows and column tile (of nt). Groups take ceil(rows / TM) row tiles each, in
+// order, the rows of no expert last; a row tile's column tiles follow each other, and each XCD gets one range of the
+// tiles that there are (of the grid's, which allows every group a part tile, the last XCDs' would be the missing ones).
+// False past the last tile.
+template <int TM> DEV bool mx_tile(const MxMulArgs &a, int nt, int64_t &e, int64_t &r0, int64_t &r1, int &col) {
+    const int lane = lane_id();
+    int total = a.mt;
+    if (a.offsets) {
+        total = 0;
+        for (int64_t g0 = 0; g0 <= a.nmat; g0 += 64) {
+            int64_t s0 = 0, s1 = 0;
+            if (g0 + lane <= a.nmat) mx_group(a, g0 + lane, s0, s1);
+            total += (int)((s1 - s0 + TM - 1) / TM);
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
+        total = __builtin_amdgcn_readfirstlane(total);
+        total = total < a.mt ? total : a.mt;                // (more only of offsets that do not ascend)
+    }
+    const int per = (total * nt + 7) / 8, at = (int)(blockIdx.x / 8), id = (int)(blockIdx.x % 8) * per + at;
+    if (at >= per || id >= total * nt) return false;
+    const int t = id / nt;
+    col = id % nt;
     if (!a.offsets) {
         e = 0;
         r0 = (int64_t)t * TM;
         r1 = a.m < r0 + TM ? a.m : r0 + TM;
-        return r0 < a.m;
+        return true;
     }
-    const int lane = lane_id();
     int base = 0;
     for (int64_t g0 = 0; g0 <= a.nmat; g0 += 64) {
         int64_t s0 = 0, s1 = 0;
@@ -236,14 +320,14 @@ template <int TM> DEV bool mx_tile(const MxMulArgs &a, int t, int64_t &e, int64_
         const uint64_t here = __ballot(base + inc > t);
         if (here) {
             const int l = __ffsll((unsigned long long)here) - 1;
-            const int skip = base + __shfl(inc, l, 64) - __shfl(cnt, l, 64);
-            const int s0i = __shfl((int)s0, l, 64), s1i = __shfl((int)s1, l, 64);
+            const int skip = base + __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(cnt, l);
             e = g0 + l;
-            r0 = (int64_t)s0i + (int64_t)(t - skip) * TM;
-            r1 = r0 + TM < s1i ? r0 + TM : s1i;
+            r0 = (int64_t)__builtin_amdgcn_readlane((int)s0, l) + (int64_t)(t - skip) * TM;
+            r1 = __builtin_amdgcn_readlane((int)s1, l);
+            r1 = r0 + TM < r1 ? r0 + TM : r1;
             return true;
         }
-        base += __shfl(inc, 63, 64);
+        base += __builtin_amdgcn_readlane(inc, 63);
     }
     return false;
 }
@@ -263,33 +347,88 @@ DEV void mx_sync() {
     __syncthreads();
 }
 
-// WM x WN waves, each FM x 16 rows by FN x 16 columns (with GLU the first half of its FN strips are w's and the second
-// the same columns of u). x goes through LDS, 256 bytes of every row a step (128 BF16 values or 512 codes), in two
-// buffers: piece 4c + q of a row's 16, which lane group q takes into product c, lies at (4c + q) ^ (row & 15), so that
-// the reads of 16 rows spread over the banks. A wave's weights go straight to its registers, a kilobyte of a strip at a
-// time and one ahead: as codes they are a quarter of what BF16 rows take, and half of them are read twice.
-template <bool FP4, int WM, int WN, int FM, int FN, bool GLU>
-__global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
-    constexpr int TM = WM * FM * 16, NS = WN * FN / (GLU ? 2 : 1), NO = NS * 16, NW = WM * WN, LD = TM / 4 / NW;
-    constexpr int FH = GLU ? FN / 2 : FN;                   // strips of one matrix
-    __shared__ __align__(1024) uint8_t xs[2 * TM * 256];
-    __shared__ __align__(16) uint8_t xsc[FP4 ? 2 * TM * 16 : 16];
-    const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
-    const int nt = (int)((a.strips + NS - 1) / NS), total = nt * a.mt, per = (total + 7) / 8;
-    const int id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    if ((int)(blockIdx.x / 8) >= per || id >= total) return;
-    int64_t e, r0, r1;
-    if (!mx_tile<TM>(a, id / nt, e, r0, r1)) return;
-    const int64_t s0 = (int64_t)(id % nt) * NS;             // the tile's first strip
-    if (e == a.nmat) {
-        const float z[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t i = tid; i < (r1 - r0) * (NO / 4); i += NW * 64) {
-            const int64_t n = s0 * 16 + 4 * (i % (NO / 4));
-            if (n < a.ne1) mx_store4(a, r0 + i / (NO / 4), n, z);
+// The tile's sums leave through LDS, GC fragments of every wave at a time, so that a store writes whole lines of a row
+// (16 bytes a lane of which four lanes share a row were 14 us of the 73 that 8192 x 2048 x 7168 takes with MXFP4 rows).
+// Rows that are not whole 16-byte pieces are stored value by value. lds: the loop's buffers, free by now.
+template <int WM, int WN, int FM, int FN, bool GLU>
+DEV void mx_epilogue(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0, int64_t r1, int64_t s0, uint8_t *lds) {
+    constexpr int FH = GLU ? FN / 2 : FN, NO = WN * FH * 16, GC = FM / 4, CR = WM * GC * 16;
+    const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+    const int size = a.ytype == T_F32 ? 4 : 2, rb = NO * size + 16, per = 16 / size;
+    const bool whole = a.ne1 % per == 0;
+#pragma unroll
+    for (int g0 = 0; g0 < FM; g0 += GC) {
+#pragma unroll
+        for (int i = 0; i < GC; ++i) {
+            const int64_t r = r0 + (wm * FM + g0 + i) * 16 + (lane & 15);
+            const bool on = r < r1 && mx_row(a, r) >= 0;
+            uint8_t *l = lds + ((wm * GC + i) * 16 + (lane & 15)) * rb + (wn * FH * 16 + 4 * q) * size;
+#pragma unroll
+            for (int f = 0; f < FH; ++f) {
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[k] = acc[f][g0 + i][k];
+                    if (GLU) v[k] = mx_glu(v[k], acc[(f + FH) % FN][g0 + i][k]);
+                    if (!on) v[k] = 0.f;
+                }
+                if (!whole) {
+                    const int64_t n = (s0 + wn * FH + f) * 16 + 4 * q;
+                    if (r < r1 && n < a.ne1) mx_store4(a, r, n, v);
+                } else if (size == 4) {
+                    *(float4 *)(l + f * 64) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) h[k] = a.ytype == T_BF16 ? mx_bf16(v[k]) : mx_f16(v[k]);
+                    *(uint2 *)(l + f * 32) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+                }
+            }
         }
-        return;
+        if (!whole) continue;                               // (uniform)
+        __syncthreads();
+        const int pieces = NO / per;                        // of a row
+        for (int i = tid; i < CR * pieces; i += WM * WN * 64) {
+            const int lr = i / pieces, p = i % pieces, w = lr / (GC * 16);
+            const int64_t r = r0 + (w * FM + g0) * 16 + lr % (GC * 16), n = s0 * 16 + p * per;
+            if (r < r1 && n < a.ne1)
+                *(uint4 *)((uint8_t *)a.y + (r * a.ne1 + n) * size) = *(const uint4 *)(lds + lr * rb + p * 16);
+        }
+        __syncthreads();
     }
+}
+
+// BF16 rows: WN waves, each all FM x 16 rows by FN x 16 columns (with GLU the first half of its FN strips are w's and the
+// second the same columns of u). x goes through LDS, 128 values of every row a step, in two buffers: piece 4q + c of a
+// row's 16, which lane group q takes into product c, lies at (4c + q) ^ (row & 15), so that the reads of 16 rows spread
+// over the banks. A wave's weights go straight to its registers, a kilobyte of a strip at a time and one ahead: as codes
+// they are a quarter of what the rows take, and no two waves read the same.
+template <int WN, int FM, int FN, bool GLU>
+DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int64_t s0, uint8_t *xs) {
+    constexpr int TM = FM * 16, FH = GLU ? FN / 2 : FN, LD = TM / 4 / WN, HP = FM / 2;
+    const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint8_t *wp[FN], *wsp[FN];        // (uniform) this wave's strips, those past the last the last
+#pragma unroll
+    for (int f = 0; f < FN; ++f) {
+        const int64_t t = s0 + wave * FH + f % FH, strip = e * a.strips + (t < a.strips ? t : a.strips - 1);
+        wp[f] = (f < FH ? a.w : a.u) + strip * a.nc * 4096;
+        wsp[f] = (f < FH ? a.ws : a.us) + strip * a.nc * 256;
+    }
+    uint4 wq[FN], wn[FN];
+    uint32_t sc[FN], sn[FN];
+    auto fetch = [&](int c) {               // the weights' piece c
+        const uint32_t at = mx_opaque(16u * (uint32_t)lane);
+#pragma unroll
+        for (int f = 0; f < FN; ++f) wn[f] = *(const uint4 *)(wp[f] + (int64_t)c * 1024 + at);
+    };
+    auto scales = [&](int c) {              // and the scales of its 512 values
+        const uint32_t at = mx_opaque(4u * (uint32_t)lane);
+#pragma unroll
+        for (int f = 0; f < FN; ++f) sn[f] = *(const uint32_t *)(wsp[f] + (int64_t)c * 256 + at);
+    };
+    fetch(0);
+    scales(0);
     // where this lane's 16-byte pieces of x come from
     const uint8_t *xp[LD];
 #pragma unroll
@@ -298,31 +437,18 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
         const int64_t r = r0 + row < r1 ? r0 + row : r1 - 1;
         const int64_t j = mx_row(a, r);
         const int p = (lane & 15) ^ (row & 15);
-        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * (FP4 ? p : 4 * (p & 3) + (p >> 2));
-    }
-    const uint8_t *sp = a.xs;               // FP4: a row's scales of 512 values, a lane each of the first TM
-    if (FP4) {
-        const int64_t r = r0 + tid < r1 ? r0 + tid : r1 - 1;
-        const int64_t j = mx_row(a, r);
-        sp += (j < 0 ? 0 : j) * 16;
-    }
-    const uint8_t *wp[FN], *wsp[FN];        // (uniform) this wave's strips, those past the last the last
-#pragma unroll
-    for (int f = 0; f < FN; ++f) {
-        const int64_t t = s0 + wn * FH + f % FH, strip = e * a.strips + (t < a.strips ? t : a.strips - 1);
-        wp[f] = (f < FH ? a.w : a.u) + strip * a.nc * 4096;
-        wsp[f] = (f < FH ? a.ws : a.us) + strip * a.nc * 256;
+        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * (4 * (p & 3) + (p >> 2));
     }
     mx_f4 acc[FN][FM];
 #pragma unroll
     for (int f = 0; f < FN; ++f)
 #pragma unroll
         for (int g = 0; g < FM; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
-    const int steps = FP4 ? a.nc : a.nk * a.pieces;
+    const int steps = a.nk * a.pieces;
     // part j of 4 of step s into its buffer
     auto stage = [&](int s, int j) {
         uint8_t *buf = xs + (s & 1) * (TM * 256);
-        if (!FP4 && (int64_t)s * 128 + 128 > a.kx) {        // (the last step, of rows that end inside it)
+        if ((int64_t)s * 128 + 128 > a.kx) {                // (the last step, of rows that end inside it)
 #pragma unroll
             for (int i = j * LD / 4; i < (j + 1) * LD / 4; ++i) {
                 const int p = (lane & 15) ^ (((wave * LD + i) * 4 + (lane >> 4)) & 15);
@@ -336,102 +462,204 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mx_tile(MxMulArgs a) {
                 xp[i] += 256;
             }
         }
-        if (FP4 && j == 3 && wave * 64 < TM) mx_to_lds(sp + (int64_t)s * a.nx * 16, xsc + (s & 1) * (TM * 16) + wave * 1024);
     };
-    uint4 wq[FN], wn_[FN];
-    uint32_t sc[FN], sn[FN];
-    auto fetch = [&](int c) {               // the weights' piece c
-#pragma unroll
-        for (int f = 0; f < FN; ++f) wn_[f] = *(const uint4 *)(wp[f] + (int64_t)c * 1024 + 16 * lane);
-    };
-    auto scales = [&](int c) {              // and the scales of its 512 values
-#pragma unroll
-        for (int f = 0; f < FN; ++f) sn[f] = *(const uint32_t *)(wsp[f] + (int64_t)c * 256 + 4 * lane);
-    };
-    int c = 0;                              // BF16: the piece at hand
+    int c = 0;                              // the piece at hand
 #pragma unroll
     for (int j = 0; j < 4; ++j) stage(0, j);
-    fetch(0);
-    scales(0);
     mx_sync();
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
-        const uint8_t *b = xs + (s & 1) * (TM * 256) + (wm * FM * 16 + (lane & 15)) * 256;
+        const uint8_t *b = xs + (s & 1) * (TM * 256) + (lane & 15) * 256;
         const bool more = s + 1 < steps;
-        uint32_t xc[FP4 ? FM : 1];
-        const int next = FP4 ? s + 1 : c + 1 < a.nk ? c + 1 : 0;
-        if (FP4) {
+        const int next = c + 1 < a.nk ? c + 1 : 0;          // (F16 and F32 rows: the weights start over with each piece)
 #pragma unroll
-            for (int g = 0; g < FM; ++g)
-                xc[g] = *(const uint32_t *)(xsc + (s & 1) * (TM * 16) + ((wm * FM + g) * 16 + (lane & 15)) * 16 + 4 * q);
-#pragma unroll
-            for (int f = 0; f < FN; ++f) sc[f] = sn[f];
-            if (more) scales(next);
-        } else {
-#pragma unroll
-            for (int f = 0; f < FN; ++f) {
-                wq[f] = wn_[f];
-                sc[f] = ((sn[f] >> (8 * (c & 3))) & 255) << 23;
-            }
-            if (more) {
-                fetch(next);
-                if ((next & 3) == 0) scales(next >> 2);
-            }
+        for (int f = 0; f < FN; ++f) {
+            wq[f] = wn[f];
+            sc[f] = ((sn[f] >> (8 * (c & 3))) & 255) << 23;
         }
+        if (more) {
+            fetch(next);
+            if ((next & 3) == 0) scales(next >> 2);
+        }
+        // two fragments of x at a time, the next two on their way
+        uint4 xv[2][2];
+        auto read = [&](int t) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (FP4) {
-                if (4 * s + j >= a.nk) continue;            // (padding)
+            for (int i = 0; i < 2; ++i)
+                xv[t & 1][i] = *(const uint4 *)(b + (t % HP * 2 + i) * 4096 + (((4 * (t / HP) + q) ^ (lane & 15)) * 16));
+        };
+        mx_bf8 wv[FN];
 #pragma unroll
-                for (int f = 0; f < FN; ++f) wq[f] = wn_[f];
-                if (j < 3 || more) fetch(4 * s + j + 1);    // (the last piece of a row is followed by its scales at least)
-            }
-            if (more) stage(s + 1, j);
-            mx_bf8 wv[FN];
-            if (!FP4) {
+        for (int t = 0; t < 4 * HP; ++t) {
+            const int j = t / HP, p = t % HP;
+            if (t == 0) read(t);
+            if (t + 1 < 4 * HP) read(t + 1);
+            if (p == 0) {
 #pragma unroll
                 for (int f = 0; f < FN; ++f)
                     wv[f] = mx_widen(j == 0 ? wq[f].x : j == 1 ? wq[f].y : j == 2 ? wq[f].z : wq[f].w, ffrom(sc[f]));
+                if (more) stage(s + 1, j);
             }
 #pragma unroll
-            for (int g = 0; g < FM; ++g) {
-                const uint4 xv = *(const uint4 *)(b + g * 4096 + (((4 * j + q) ^ (lane & 15)) * 16));
-                union { uint4 u; mx_bf8 b; } xb = {xv};
+            for (int i = 0; i < 2; ++i) {
+                union { uint4 u; mx_bf8 b; } x = {xv[t & 1][i]};
 #pragma unroll
-                for (int f = 0; f < FN; ++f) {
-                    if (FP4) {
-                        const mx_i8 wi = mx_wide(wq[f]), xi = mx_wide(xv);
-                        const int ws = (int)sc[f], xw = (int)xc[FP4 ? g : 0];
-                        acc[f][g] = j == 0   ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wi, xi, acc[f][g], 4, 4, 0, ws, 0, xw)
-                                    : j == 1 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wi, xi, acc[f][g], 4, 4, 1, ws, 1, xw)
-                                    : j == 2 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wi, xi, acc[f][g], 4, 4, 2, ws, 2, xw)
-                                             : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wi, xi, acc[f][g], 4, 4, 3, ws, 3, xw);
-                    } else {
-                        acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[f], xb.b, acc[f][g], 0, 0, 0);
-                    }
-                }
+                for (int f = 0; f < FN; ++f)
+                    acc[f][2 * p + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[f], x.b, acc[f][2 * p + i], 0, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (!FP4) c = next;
+        c = next;
         mx_sync();
     }
+    mx_epilogue<1, WN, FM, FN, GLU>(a, acc, r0, r1, s0, xs);
+}
+
+// Tiles of FM x 16 rows; one with no more than half of them takes half the fragments
+template <int WN, int FM, int FN, bool GLU>
+__global__ __launch_bounds__(WN * 64) __attribute__((amdgpu_waves_per_eu(2))) void k_mx_tile(MxMulArgs a) {
+    constexpr int NS = WN * FN / (GLU ? 2 : 1);
+    __shared__ __align__(1024) uint8_t xs[2 * FM * 16 * 256];
+    int64_t e, r0, r1;
+    int col;
+    if (!mx_tile<FM * 16>(a, (int)((a.strips + NS - 1) / NS), e, r0, r1, col)) return;
+    const int64_t s0 = (int64_t)col * NS;                   // the tile's first strip
+    if (e == a.nmat) mx_clear<NS * 16>(a, r0, r1, s0 * 16, WN * 64);
+    else if (FM == 8 && r1 - r0 <= FM * 8) mx_tile_body<WN, FM == 8 ? FM / 2 : FM, FN, GLU>(a, e, r0, r1, s0, xs);
+    else mx_tile_body<WN, FM, FN, GLU>(a, e, r0, r1, s0, xs);
+}
+
+// MXFP4 rows: WM x WN waves, each FM x 16 rows by FN x 16 columns. Both sides are codes and as large, and the products
+// take a quarter of the BF16 ones' time, so both go through LDS (nothing is read twice), 256 values of k a step in two
+// buffers, and every load has a step's time. A row of x is 8 pieces of 16 bytes, piece p at p ^ (row / 2 & 7); a strip's
+// kilobytes lie as they are stored. The scales of 512 values follow every second step.
+template <int WM, int WN, int FM, int FN, bool GLU>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2))) void k_mx_tile4(MxMulArgs a) {
+    constexpr int TM = WM * FM * 16, FH = GLU ? FN / 2 : FN, NS = WN * FH, NO = NS * 16, NW = WM * WN, TS = WN * FN;
+    constexpr int LX = TM / 8 / NW, LW = TS * 2 / NW, XB = TM * 128, WB = TS * 2048;
+    static_assert(LX * 8 * NW == TM && LW * NW == TS * 2, "whole loads");
+    __shared__ __align__(1024) uint8_t buf[2 * (XB + WB)];
+    __shared__ __align__(1024) uint8_t scl[2 * (TM * 16 + TS * 256)];
+    const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+    int64_t e, r0, r1;
+    int col;
+    if (!mx_tile<TM>(a, (int)((a.strips + NS - 1) / NS), e, r0, r1, col)) return;
+    const int64_t s0 = (int64_t)col * NS;
+    if (e == a.nmat) {
+        mx_clear<NO>(a, r0, r1, s0 * 16, NW * 64);
+        return;
+    }
+    // strip t of the tile: those of wave column v are its FH of w and, with GLU, the same FH of u
+    auto strip = [&](int t) {
+        const int64_t k = s0 + t / FN * FH + t % FN % FH;
+        return e * a.strips + (k < a.strips ? k : a.strips - 1);
+    };
+    const uint8_t *xp[LX], *wp[LW];
 #pragma unroll
-    for (int g = 0; g < FM; ++g) {
-        const int64_t r = r0 + (wm * FM + g) * 16 + (lane & 15);
-        if (r >= r1) continue;
-        const bool on = mx_row(a, r) >= 0;
+    for (int i = 0; i < LX; ++i) {
+        const int row = (wave * LX + i) * 8 + (lane >> 3);
+        const int64_t r = r0 + row < r1 ? r0 + row : r1 - 1;
+        const int64_t j = mx_row(a, r);
+        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * ((lane & 7) ^ ((row >> 1) & 7));
+    }
 #pragma unroll
-        for (int f = 0; f < FH; ++f) {
-            const int64_t n = (s0 + wn * FH + f) * 16 + 4 * q;
-            float v[4];
+    for (int i = 0; i < LW; ++i) {                          // (uniform: kilobyte h of strip t)
+        const int t = (wave * LW + i) / 2, h = (wave * LW + i) % 2;
+        wp[i] = (t % FN < FH ? a.w : a.u) + strip(t) * a.nc * 4096 + h * 1024;
+    }
+    // scales: a lane takes one row's 16 bytes, or 16 of the 256 of a strip; wave by wave, rows first
+    constexpr int SX = TM / 64, SI = (SX + TS / 4 + NW - 1) / NW;
+    const uint8_t *sp[SI];
+    int64_t sstep[SI];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = acc[f][g][i];
-                if (GLU) v[i] = mx_glu(v[i], acc[(f + FH) % FN][g][i]);
-                if (!on) v[i] = 0.f;
-            }
-            if (n < a.ne1) mx_store4(a, r, n, v);
+    for (int i = 0; i < SI; ++i) {
+        const int k = wave + i * NW;
+        if (k < SX) {
+            const int64_t r = r0 + k * 64 + lane < r1 ? r0 + k * 64 + lane : r1 - 1;
+            const int64_t j = mx_row(a, r);
+            sp[i] = a.xs + (j < 0 ? 0 : j) * 16;
+            sstep[i] = a.nx * 16;
+        } else {
+            const int t = (k - SX) * 4 + (lane >> 4) < TS ? (k - SX) * 4 + (lane >> 4) : TS - 1;
+            sp[i] = (t % FN < FH ? a.ws : a.us) + strip(t) * a.nc * 256 + (lane & 15) * 16;
+            sstep[i] = 256;
         }
     }
+    mx_f4 acc[FN][FM];
+#pragma unroll
+    for (int f = 0; f < FN; ++f)
+#pragma unroll
+        for (int g = 0; g < FM; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
+    const int steps = (a.nk + 1) / 2;
+    auto stage = [&](int s) {
+        uint8_t *x = buf + (s & 1) * (XB + WB), *w = x + XB;
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            mx_to_lds(xp[i], x + (wave * LX + i) * 1024);
+            xp[i] += 128;
+        }
+        const uint32_t at = mx_opaque(16u * (uint32_t)lane);
+#pragma unroll
+        for (int i = 0; i < LW; ++i) mx_to_lds(wp[i] + (int64_t)s * 2048 + at, w + (wave * LW + i) * 1024);
+        if ((s & 1) == 0) {
+#pragma unroll
+            for (int i = 0; i < SI; ++i) {
+                const int k = wave + i * NW;
+                if (k < SX + TS / 4) mx_to_lds(sp[i], scl + ((s >> 1) & 1) * (TM * 16 + TS * 256) + k * 1024);
+                sp[i] += sstep[i];
+            }
+        }
+    };
+    const int sw = (lane >> 1) & 7;
+    uint32_t xc[FM], wc[FN];
+    stage(0);
+    mx_sync();
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+        const uint8_t *x = buf + (s & 1) * (XB + WB) + (wm * FM * 16 + (lane & 15)) * 128;
+        const uint8_t *w = buf + (s & 1) * (XB + WB) + XB + wn * FN * 2048 + 16 * lane;
+        if (s + 1 < steps) stage(s + 1);
+        if ((s & 1) == 0) {
+            const uint8_t *c = scl + ((s >> 1) & 1) * (TM * 16 + TS * 256);
+#pragma unroll
+            for (int g = 0; g < FM; ++g) xc[g] = *(const uint32_t *)(c + ((wm * FM + g) * 16 + (lane & 15)) * 16 + 4 * q);
+#pragma unroll
+            for (int f = 0; f < FN; ++f) wc[f] = *(const uint32_t *)(c + TM * 16 + (wn * FN + f) * 256 + 4 * lane);
+        } else {
+#pragma unroll
+            for (int g = 0; g < FM; ++g) xc[g] >>= 16;
+#pragma unroll
+            for (int f = 0; f < FN; ++f) wc[f] >>= 16;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint4 wv[FN], xv[2][2];
+            auto read = [&](int p) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) xv[p & 1][i] = *(const uint4 *)(x + (2 * p + i) * 2048 + ((4 * h + q) ^ sw) * 16);
+            };
+#pragma unroll
+            for (int f = 0; f < FN; ++f) wv[f] = *(const uint4 *)(w + f * 2048 + h * 1024);
+            read(0);
+#pragma unroll
+            for (int p = 0; p < FM / 2; ++p) {
+                    if (p + 1 < FM / 2) read(p + 1);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int g = 2 * p + i;
+                    const mx_i8 xi = mx_wide(xv[p & 1][i]);
+#pragma unroll
+                    for (int f = 0; f < FN; ++f)
+                        acc[f][g] = h == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                                 mx_wide(wv[f]), xi, acc[f][g], 4, 4, 0, (int)wc[f], 0, (int)xc[g])
+                                           : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                                 mx_wide(wv[f]), xi, acc[f][g], 4, 4, 1, (int)wc[f], 1, (int)xc[g]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        mx_sync();
+    }
+    mx_epilogue<WM, WN, FM, FN, GLU>(a, acc, r0, r1, s0, buf);
 }
