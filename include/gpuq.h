@@ -170,8 +170,10 @@ size_t gpuq_mxfp4_bytes(int form, int64_t nmat, int64_t nrow, int64_t n_per_row)
 size_t gpuq_mxfp4_quantize_dev(int src_type, const void *d_src, int64_t nmat, int64_t nrow, int64_t n_per_row, int64_t ld,
                                int form, void *d_dst, void *d_values, void *stream);
 
-/* The scratch bytes gpuq_mxfp4_matmul_dev needs at d_work for nx rows of x_type (0 for BF16 and MXFP4: NULL will do) */
-size_t gpuq_mxfp4_matmul_work(int x_type, int64_t nx, int64_t ne0);
+/* The scratch bytes a call of gpuq_mxfp4_matmul_dev with these sizes needs at d_work (0: NULL will do); glu: with d_up,
+ * grouped: with d_offsets */
+size_t gpuq_mxfp4_matmul_work(int x_type, int glu, int64_t nx, int64_t nmat, int64_t ne1, int64_t ne0, int grouped,
+                              int64_t m);
 
 /* Products of rows with MXFP4 matrices d_w [nmat][ne1][ne0] (tiles): y[r] = x[d_rows[r]] w[e]^T for the rows
  * d_offsets[e] <= r < d_offsets[e + 1] of matrix e (int32, device; nmat 1: d_offsets may be NULL, all m rows). d_rows NULL:

@@ -36,6 +36,14 @@ template <int SRC> void launch_quantize(int form, const MxQuantArgs &p, hipStrea
 int pieces_of(int x_type) { return x_type == T_F32 ? 3 : x_type == T_F16 ? 2 : 1; }
 int64_t round128(int64_t n) { return (n + 127) / 128 * 128; }
 
+size_t pieces_bytes(int x_type, int64_t nx, int64_t ne0) {
+    return pieces_of(x_type) > 1 ? (size_t)(nx * pieces_of(x_type) * round128(ne0) * 2) : 0;
+}
+bool sizes_ok(int64_t nx, int64_t nmat, int64_t ne1, int64_t ne0, int64_t m) {
+    return nmat > 0 && nmat <= 65534 && ne1 > 0 && ne1 <= MAX_ROWS && nmat * strips_of(ne1) <= MAX_ROWS && cols_ok(ne0) &&
+           nx > 0 && nx <= MAX_ROWS && m > 0 && m <= MAX_ROWS;
+}
+
 template <int MF, int NF> void launch_rows(bool fp4, bool glu, const MxMulArgs &a, hipStream_t st) {
     const dim3 grid((unsigned)((a.strips + NF - 1) / NF), (unsigned)(a.offsets ? std::min(a.nmat, a.m) + 1 : 1));
 #define MX_ROWS_K(F, G) hipLaunchKernelGGL((k_mx_rows<F, MF, NF, G>), grid, dim3(512), 0, st, a)
@@ -49,29 +57,42 @@ template <int MF, int NF> void launch_rows(bool fp4, bool glu, const MxMulArgs &
 #undef MX_ROWS_K
 }
 
-// the row tiles of the grid and its workgroups, 0 for too many
-template <int TM, int TN> int64_t tile_grid(bool glu, MxMulArgs &a) {
-    const int64_t ns = TN / 16 / (glu ? 2 : 1), nt = (a.strips + ns - 1) / ns;
-    const int64_t mt = (a.m + TM - 1) / TM + (a.offsets ? a.nmat + 1 : 0);
-    if (nt * mt >= ((int64_t)1 << 30)) return 0;
-    a.mt = (int)mt;
-    return (nt * mt + 7) / 8 * 8;
+// How a product runs. A workgroup of k_mx_rows reads its strips' weights once for every 16 rows of a group: right for
+// groups of a few rows. The tile kernels read them once for 64 to 256, and where their tiles are fewer than the GPU takes
+// at once, split k and join the partial sums.
+struct Plan {
+    int kind;                   // 0 k_mx_rows; tiles of 64 (1) or 128 (2) BF16 rows, 128 (3) or 256 (4) MXFP4 rows
+    int tm, tn;
+    int64_t mt, nt;             // row and column tiles
+    int split;
+    size_t part;                // bytes of partial sums
+};
+
+bool plan_product(int x_type, bool glu, int64_t nmat, int64_t ne1, int64_t ne0, int64_t m, bool grouped, Plan &p) {
+    const bool fp4 = x_type == T_MXFP4;
+    const int64_t cols = strips_of(ne1) * (glu ? 2 : 1), some = std::min(nmat, m), per = m / some;
+    p = Plan{0, 16, 16, 0, 0, 1, 0};
+    if (grouped ? m <= 8 * nmat : m <= 16) return true;
+    auto tiles = [&](int64_t tm, int64_t tn) { return ((m + tm - 1) / tm + (some - 1) / 2) * ((cols * 16 + tn - 1) / tn); };
+    if (fp4) p.kind = per >= 256 && tiles(256, 256) >= 256 ? 4 : 3;
+    else p.kind = tiles(128, 256) >= 1024 ? 2 : 1;
+    p.tm = p.kind == 1 ? 64 : p.kind == 4 ? 256 : 128;
+    p.tn = p.kind == 3 ? 128 : 256;
+    p.nt = (cols * 16 + p.tn - 1) / p.tn;
+    p.mt = (m + p.tm - 1) / p.tm + (grouped ? nmat + 1 : 0);
+    const int64_t n = tiles(p.tm, p.tn), steps = fp4 ? mx_padded(ne0) / 512 : round128(ne0) / 128 * pieces_of(x_type);
+    if (n < 256) p.split = (int)std::max<int64_t>(1, std::min((512 + n - 1) / n, fp4 ? steps / 2 : steps / 4));
+    if (p.split > 1) p.part = (size_t)(p.split * (glu ? 2 : 1) * m * ne1 * 4);
+    return p.nt * p.mt < ((int64_t)1 << 30);
 }
 
-template <int WN, int FM, int FN> bool launch_tile(bool glu, MxMulArgs &a, hipStream_t st) {
-    const int64_t grid = tile_grid<FM * 16, WN * FN * 16>(glu, a);
-    if (!grid) return false;
-    if (glu) hipLaunchKernelGGL((k_mx_tile<WN, FM, FN, true>), dim3((unsigned)grid), dim3(WN * 64), 0, st, a);
-    else hipLaunchKernelGGL((k_mx_tile<WN, FM, FN, false>), dim3((unsigned)grid), dim3(WN * 64), 0, st, a);
-    return true;
+template <int WN, int FM, int FN> void launch_tile(bool glu, dim3 grid, const MxMulArgs &a, hipStream_t st) {
+    if (glu) hipLaunchKernelGGL((k_mx_tile<WN, FM, FN, true>), grid, dim3(WN * 64), 0, st, a);
+    else hipLaunchKernelGGL((k_mx_tile<WN, FM, FN, false>), grid, dim3(WN * 64), 0, st, a);
 }
-
-template <int WM, int WN, int FM, int FN> bool launch_tile4(bool glu, MxMulArgs &a, hipStream_t st) {
-    const int64_t grid = tile_grid<WM * FM * 16, WN * FN * 16>(glu, a);
-    if (!grid) return false;
-    if (glu) hipLaunchKernelGGL((k_mx_tile4<WM, WN, FM, FN, true>), dim3((unsigned)grid), dim3(WM * WN * 64), 0, st, a);
-    else hipLaunchKernelGGL((k_mx_tile4<WM, WN, FM, FN, false>), dim3((unsigned)grid), dim3(WM * WN * 64), 0, st, a);
-    return true;
+template <int WM, int WN, int FM, int FN> void launch_tile4(bool glu, dim3 grid, const MxMulArgs &a, hipStream_t st) {
+    if (glu) hipLaunchKernelGGL((k_mx_tile4<WM, WN, FM, FN, true>), grid, dim3(WM * WN * 64), 0, st, a);
+    else hipLaunchKernelGGL((k_mx_tile4<WM, WN, FM, FN, false>), grid, dim3(WM * WN * 64), 0, st, a);
 }
 
 template <int SRC> bool launch_route(const RouteArgs &a, hipStream_t st) {
@@ -153,9 +174,13 @@ extern "C" size_t gpuq_mxfp4_quantize_dev(int src_type, const void *d_src, int64
     return size;
 }
 
-extern "C" size_t gpuq_mxfp4_matmul_work(int x_type, int64_t nx, int64_t ne0) {
-    if (pieces_of(x_type) == 1 || nx <= 0 || nx > MAX_ROWS || !cols_ok(ne0)) return 0;
-    return (size_t)(nx * pieces_of(x_type) * round128(ne0) * 2);
+extern "C" size_t gpuq_mxfp4_matmul_work(int x_type, int glu, int64_t nx, int64_t nmat, int64_t ne1, int64_t ne0,
+                                         int grouped, int64_t m) {
+    Plan p;
+    if ((x_type != T_MXFP4 && !float_type(x_type)) || !sizes_ok(nx, nmat, ne1, ne0, m) ||
+        !plan_product(x_type, glu != 0, nmat, ne1, ne0, m, grouped != 0, p))
+        return 0;
+    return pieces_bytes(x_type, nx, ne0) + p.part;
 }
 
 extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx, int64_t ld, const void *d_w,
@@ -164,15 +189,17 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
                                         void *d_y, void *d_work, void *stream) {
     const bool fp4 = x_type == T_MXFP4;
     if (gq_device() < 0 || !d_x || !d_w || !d_y || (!fp4 && !float_type(x_type)) || !float_type(y_type)) return 0;
-    if (nmat <= 0 || nmat > 65534 || nmat * strips_of(ne1) > MAX_ROWS || ne1 <= 0 || ne1 > MAX_ROWS || !cols_ok(ne0) || nx <= 0 || nx > MAX_ROWS || m <= 0 ||
-        m > MAX_ROWS || (nmat > 1 && !d_offsets) || (!d_rows && m > nx))
-        return 0;
+    if (!sizes_ok(nx, nmat, ne1, ne0, m) || (nmat > 1 && !d_offsets) || (!d_rows && m > nx)) return 0;
     if (!aligned16(d_x) || !aligned16(d_w) || !aligned16(d_up) || !aligned16(d_y) || ((uintptr_t)d_offsets & 3) ||
         ((uintptr_t)d_rows & 3))
         return 0;
     if (fp4 ? ld != ne0 : ld < ne0 || ld > ((int64_t)1 << 40) || ld * type_size(x_type) % 16) return 0;
     const int pieces = pieces_of(x_type);
-    if (pieces > 1 && (!d_work || !aligned16(d_work))) return 0;
+    const bool glu = d_up != nullptr;
+    Plan plan;
+    if (!plan_product(x_type, glu, nmat, ne1, ne0, m, d_offsets != nullptr, plan)) return 0;
+    const size_t px = pieces_bytes(x_type, nx, ne0);
+    if ((px + plan.part) && (!d_work || !aligned16(d_work))) return 0;
     const hipStream_t st = (hipStream_t)stream;
     const int64_t np = mx_padded(ne0), strips = strips_of(ne1), wcodes = nmat * strips * 8 * np;
     MxMulArgs a = {};
@@ -211,15 +238,20 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
         a.xrow = kp * 2 * pieces;
         a.kx = kp * pieces;
     }
-    const bool glu = d_up != nullptr;
-    const int64_t per = m / nmat;                               // rows a group, on average
-    const int64_t tiles = (m + 127) / 128 * ((strips * (glu ? 2 : 1) + 15) / 16);       // 128 x 256
-    if (per <= 16) launch_rows<1, 1>(fp4, glu, a, st);
-    else if (per <= 64) launch_rows<4, 1>(fp4, glu, a, st);
-    else if (fp4) {
-        if (per < 256 ? !launch_tile4<2, 4, 4, 2>(glu, a, st) : !launch_tile4<2, 4, 8, 4>(glu, a, st)) return 0;
-    } else if (tiles < 1024 ? !launch_tile<4, 4, 4>(glu, a, st) : !launch_tile<4, 8, 4>(glu, a, st)) {
-        return 0;
+    if (plan.kind == 0) {
+        // four strips a workgroup where that leaves two for every CU
+        if (a.strips * std::min(nmat, m) >= 2048) launch_rows<1, 4>(fp4, glu, a, st);
+        else launch_rows<1, 1>(fp4, glu, a, st);
+    } else {
+        a.mt = (int)plan.mt;
+        a.part = plan.split > 1 ? (float *)((uint8_t *)d_work + px) : nullptr;
+        const dim3 grid((unsigned)((plan.nt * plan.mt + 7) / 8 * 8), (unsigned)plan.split);
+        if (plan.kind == 1) launch_tile<4, 4, 4>(glu, grid, a, st);
+        else if (plan.kind == 2) launch_tile<4, 8, 4>(glu, grid, a, st);
+        else if (plan.kind == 3) launch_tile4<2, 4, 4, 2>(glu, grid, a, st);
+        else launch_tile4<2, 4, 8, 4>(glu, grid, a, st);
+        if (a.part)
+            hipLaunchKernelGGL(k_mx_join, dim3((unsigned)((m * ((ne1 + 3) / 4) + 255) / 256)), dim3(256), 0, st, a, plan.split);
     }
     return hipGetLastError() == hipSuccess ? (size_t)(m * ne1 * type_size(y_type)) : 0;
 }

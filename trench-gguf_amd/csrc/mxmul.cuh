@@ -28,6 +28,7 @@ struct MxMulArgs {
     void *y;
     int ytype;
     int mt;                     // row tiles of the grid (an upper bound with offsets)
+    float *part;                // partial sums [split][1, with SwiGLU 2][m][ne1] of tiles whose k the grid's y splits, or null
 };
 
 static __device__ __align__(16) uint32_t mx_zero[4];
@@ -102,12 +103,58 @@ DEV mx_bf8 mx_widen(uint32_t codes, float s) {
 
 DEV mx_i8 mx_wide(uint4 v) { return mx_i8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
 
+// four partial sums of product h (0 of w, 1 of u), the part of them that is there
+DEV void mx_part4(const MxMulArgs &a, int h, int64_t row, int64_t n, const float (&v)[4]) {
+    float *y = a.part + (((int64_t)blockIdx.y * (a.u ? 2 : 1) + h) * a.m + row) * a.ne1 + n;
+    if (a.ne1 % 4 == 0) {
+        *(float4 *)y = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < a.ne1) y[i] = v[i];
+    }
+}
+
+// the sum of the partial sums, in order; a thread 4 outputs of a row, a row's pieces beyond its end left out
+__global__ __launch_bounds__(256) void k_mx_join(MxMulArgs a, int split) {
+    const int64_t per = (a.ne1 + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.m * per) return;
+    const int64_t row = i / per, n = i % per * 4, plane = a.m * a.ne1;
+    const int mats = a.u ? 2 : 1;
+    float v[2][4] = {};
+    for (int z = 0; z < split; ++z) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h >= mats) continue;
+            const float *p = a.part + ((int64_t)z * mats + h) * plane + row * a.ne1 + n;
+            if (a.ne1 % 4 == 0) {
+                const float4 q = *(const float4 *)p;
+                v[h][0] += q.x; v[h][1] += q.y; v[h][2] += q.z; v[h][3] += q.w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (n + k < a.ne1) v[h][k] += p[k];
+            }
+        }
+    }
+    if (a.u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[0][k] = mx_glu(v[0][k], v[1][k]);
+    }
+    mx_store4(a, row, n, v[0]);
+}
+
 // rows that no group has: zeros, in NO columns from n0 on
 template <int NO> DEV void mx_clear(const MxMulArgs &a, int64_t r0, int64_t r1, int64_t n0, int threads) {
     const float z[4] = {0.f, 0.f, 0.f, 0.f};
     for (int64_t i = threadIdx.x; i < (r1 - r0) * (NO / 4); i += threads) {
-        const int64_t n = n0 + 4 * (i % (NO / 4));
-        if (n < a.ne1) mx_store4(a, r0 + i / (NO / 4), n, z);
+        const int64_t n = n0 + 4 * (i % (NO / 4)), r = r0 + i / (NO / 4);
+        if (n >= a.ne1) continue;
+        if (!a.part) {
+            mx_store4(a, r, n, z);
+        } else {
+            for (int h = 0; h < (a.u ? 2 : 1); ++h) mx_part4(a, h, r, n, z);
+        }
     }
 }
 
@@ -156,7 +203,7 @@ DEV bool mx_group_at(const MxMulArgs &a, int y, int64_t &e, int64_t &r0, int64_t
 
 template <bool FP4, int MF, int NF, bool GLU>
 __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
-    constexpr int G = NF * (GLU ? 2 : 1), D = MF == 1 ? 3 : 2;      // streams of weights; pieces in flight
+    constexpr int G = NF * (GLU ? 2 : 1), D = 2;      // streams of weights; pieces in flight
     __shared__ mx_f4 red[8][MF * G][64];
     const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -233,14 +280,14 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
                 }
             }
         };
-        // (a load past the end is of the last piece and not used)
 #pragma unroll
-        for (int d = 0; d < D - 1; ++d) load(wave + 8 * d < total ? wave + 8 * d : total - 1, d);
+        for (int d = 0; d < D - 1; ++d)
+            if (wave + 8 * d < total) load(wave + 8 * d, d);
         for (int s = wave; s < total; s += 8 * D) {
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 const int ahead = s + 8 * (d + D - 1);
-                load(ahead < total ? ahead : total - 1, (d + D - 1) % D);
+                if (ahead < total) load(ahead, (d + D - 1) % D);
                 if (s + 8 * d < total) work(d);
             }
         }
@@ -354,6 +401,23 @@ template <int WM, int WN, int FM, int FN, bool GLU>
 DEV void mx_epilogue(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0, int64_t r1, int64_t s0, uint8_t *lds) {
     constexpr int FH = GLU ? FN / 2 : FN, NO = WN * FH * 16, GC = FM / 4, CR = WM * GC * 16;
     const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+    if (a.part) {
+#pragma unroll
+        for (int g = 0; g < FM; ++g) {
+            const int64_t r = r0 + (wm * FM + g) * 16 + (lane & 15);
+            if (r >= r1) continue;
+            const bool on = mx_row(a, r) >= 0;
+#pragma unroll
+            for (int f = 0; f < FN; ++f) {
+                const int64_t n = (s0 + wn * FH + f % FH) * 16 + 4 * q;
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = on ? acc[f][g][k] : 0.f;
+                if (n < a.ne1) mx_part4(a, f / FH, r, n, v);
+            }
+        }
+        return;
+    }
     const int size = a.ytype == T_F32 ? 4 : 2, rb = NO * size + 16, per = 16 / size;
     const bool whole = a.ne1 % per == 0;
 #pragma unroll
@@ -408,6 +472,10 @@ DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int
     constexpr int TM = FM * 16, FH = GLU ? FN / 2 : FN, LD = TM / 4 / WN, HP = FM / 2;
     const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // this workgroup's share of the steps
+    const int all = a.nk * a.pieces, first = (int)((int64_t)all * blockIdx.y / gridDim.y);
+    const int steps = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
+    int c = first % a.nk;                   // the weights' piece at hand
     const uint8_t *wp[FN], *wsp[FN];        // (uniform) this wave's strips, those past the last the last
 #pragma unroll
     for (int f = 0; f < FN; ++f) {
@@ -427,8 +495,8 @@ DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int
 #pragma unroll
         for (int f = 0; f < FN; ++f) sn[f] = *(const uint32_t *)(wsp[f] + (int64_t)c * 256 + at);
     };
-    fetch(0);
-    scales(0);
+    fetch(c);
+    scales(c >> 2);
     // where this lane's 16-byte pieces of x come from
     const uint8_t *xp[LD];
 #pragma unroll
@@ -437,14 +505,13 @@ DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int
         const int64_t r = r0 + row < r1 ? r0 + row : r1 - 1;
         const int64_t j = mx_row(a, r);
         const int p = (lane & 15) ^ (row & 15);
-        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * (4 * (p & 3) + (p >> 2));
+        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + (int64_t)first * 256 + 16 * (4 * (p & 3) + (p >> 2));
     }
     mx_f4 acc[FN][FM];
 #pragma unroll
     for (int f = 0; f < FN; ++f)
 #pragma unroll
         for (int g = 0; g < FM; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
-    const int steps = a.nk * a.pieces;
     // part j of 4 of step s into its buffer
     auto stage = [&](int s, int j) {
         uint8_t *buf = xs + (s & 1) * (TM * 256);
@@ -463,12 +530,11 @@ DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int
             }
         }
     };
-    int c = 0;                              // the piece at hand
 #pragma unroll
-    for (int j = 0; j < 4; ++j) stage(0, j);
+    for (int j = 0; j < 4; ++j) stage(first, j);
     mx_sync();
 #pragma unroll 1
-    for (int s = 0; s < steps; ++s) {
+    for (int s = first; s < steps; ++s) {
         const uint8_t *b = xs + (s & 1) * (TM * 256) + (lane & 15) * 256;
         const bool more = s + 1 < steps;
         const int next = c + 1 < a.nk ? c + 1 : 0;          // (F16 and F32 rows: the weights start over with each piece)
@@ -550,6 +616,10 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)
         mx_clear<NO>(a, r0, r1, s0 * 16, NW * 64);
         return;
     }
+    // this workgroup's share of the steps, whole 512s of scales
+    const int first = 2 * (int)((int64_t)a.nc * blockIdx.y / gridDim.y);
+    const int last = 2 * (int)((int64_t)a.nc * (blockIdx.y + 1) / gridDim.y);
+    const int steps = last < (a.nk + 1) / 2 ? last : (a.nk + 1) / 2;
     // strip t of the tile: those of wave column v are its FH of w and, with GLU, the same FH of u
     auto strip = [&](int t) {
         const int64_t k = s0 + t / FN * FH + t % FN % FH;
@@ -561,7 +631,7 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)
         const int row = (wave * LX + i) * 8 + (lane >> 3);
         const int64_t r = r0 + row < r1 ? r0 + row : r1 - 1;
         const int64_t j = mx_row(a, r);
-        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + 16 * ((lane & 7) ^ ((row >> 1) & 7));
+        xp[i] = a.x + (j < 0 ? 0 : j) * a.xrow + (int64_t)first * 128 + 16 * ((lane & 7) ^ ((row >> 1) & 7));
     }
 #pragma unroll
     for (int i = 0; i < LW; ++i) {                          // (uniform: kilobyte h of strip t)
@@ -585,13 +655,13 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)
             sp[i] = (t % FN < FH ? a.ws : a.us) + strip(t) * a.nc * 256 + (lane & 15) * 16;
             sstep[i] = 256;
         }
+        sp[i] += first / 2 * sstep[i];
     }
     mx_f4 acc[FN][FM];
 #pragma unroll
     for (int f = 0; f < FN; ++f)
 #pragma unroll
         for (int g = 0; g < FM; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
-    const int steps = (a.nk + 1) / 2;
     auto stage = [&](int s) {
         uint8_t *x = buf + (s & 1) * (XB + WB), *w = x + XB;
 #pragma unroll
@@ -613,10 +683,10 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)
     };
     const int sw = (lane >> 1) & 7;
     uint32_t xc[FM], wc[FN];
-    stage(0);
+    stage(first);
     mx_sync();
 #pragma unroll 1
-    for (int s = 0; s < steps; ++s) {
+    for (int s = first; s < steps; ++s) {
         const uint8_t *x = buf + (s & 1) * (XB + WB) + (wm * FM * 16 + (lane & 15)) * 128;
         const uint8_t *w = buf + (s & 1) * (XB + WB) + XB + wn * FN * 2048 + 16 * lane;
         if (s + 1 < steps) stage(s + 1);

@@ -47,7 +47,7 @@ SIGNATURES = {
     "gpuq_ldlq": (_sz, [_i, _vp, _vp, _i64, ctypes.c_double, ctypes.c_double, _i, _i, _vp, _i64, _i64, _i64, _vp]),
     "gpuq_mxfp4_bytes": (_sz, [_i, _i64, _i64, _i64]),
     "gpuq_mxfp4_quantize_dev": (_sz, [_i, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp, _vp]),
-    "gpuq_mxfp4_matmul_work": (_sz, [_i, _i64, _i64]),
+    "gpuq_mxfp4_matmul_work": (_sz, [_i, _i, _i64, _i64, _i64, _i64, _i, _i64]),
     "gpuq_mxfp4_matmul_dev": (_sz, [_i, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i, _vp, _vp,
                                     _vp]),
     "gpuq_route_dev": (_i, [_i, _vp, _i64, _i64, _i, _i, _i, _vp, _i, _i, _i, ctypes.c_float, _vp, _vp, _vp]),

@@ -114,7 +114,7 @@ def matmul(gq, x, w, group=None, up=None, out_dtype=torch.float32):
         if group.offsets.numel() != w.nmat + 1:
             raise ValueError("offsets must be one longer than the stack")
     y = torch.empty((m, w.ne1), dtype=out_dtype, device=dev)
-    size = gq.gpuq_mxfp4_matmul_work(typ, n, ncol)
+    size = gq.gpuq_mxfp4_matmul_work(typ, up is not None, n, w.nmat, w.ne1, w.ne0, group is not None, m)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     got = gq.gpuq_mxfp4_matmul_dev(typ, ptr, n, ld, w.data.data_ptr(), None if up is None else up.data.data_ptr(),
                                    w.nmat, w.ne1, w.ne0, offsets, rows, m, TYPES[out_dtype], y.data_ptr(),
