@@ -273,9 +273,14 @@ extern "C" int gpuq_route_dev(int type, const void *d_logits, int64_t ntok, int6
     return ok ? 0 : 4;
 }
 
+// assignments of a chunk: at most RG_CHUNKS chunks
+static int64_t group_chunk(int64_t n) {
+    return ((n + RG_BLOCK - 1) / RG_BLOCK + RG_CHUNKS - 1) / RG_CHUNKS * RG_BLOCK;
+}
+
 extern "C" size_t gpuq_route_group_work(int64_t n, int nexp) {
-    if (n <= RG_CHUNK || n > MAX_ROWS || nexp <= 0 || nexp > RG_MAXE) return 0;
-    return (size_t)((n + RG_CHUNK - 1) / RG_CHUNK * nexp * 4);
+    if (n <= RG_BLOCK || n > MAX_ROWS || nexp <= 0 || nexp > RG_MAXE) return 0;
+    return (size_t)((n + group_chunk(n) - 1) / group_chunk(n) * nexp * 4);
 }
 
 extern "C" int gpuq_route_group_dev(const int32_t *d_ids, int64_t ntok, int k, int nexp, int32_t *d_offsets,
@@ -284,13 +289,13 @@ extern "C" int gpuq_route_group_dev(const int32_t *d_ids, int64_t ntok, int k, i
         nexp > RG_MAXE || ntok > MAX_ROWS || ntok * k > MAX_ROWS)
         return 1;
     if (((uintptr_t)d_ids | (uintptr_t)d_offsets | (uintptr_t)d_rows | (uintptr_t)d_slots | (uintptr_t)d_work) & 3) return 1;
-    const int64_t n = ntok * k;
-    const int nchunk = (int)((n + RG_CHUNK - 1) / RG_CHUNK);
+    const int64_t n = ntok * k, chunk = group_chunk(n);
+    const unsigned nchunk = (unsigned)((n + chunk - 1) / chunk);
     if (nchunk > 1 && !d_work) return 1;
     const hipStream_t st = (hipStream_t)stream;
     if (nchunk > 1)
-        hipLaunchKernelGGL(k_group_count, dim3(nchunk), dim3(256), 0, st, d_ids, n, nexp, nchunk, (int32_t *)d_work);
-    hipLaunchKernelGGL(k_group_place, dim3(nchunk), dim3(256), 0, st, d_ids, n, k, nexp, nchunk,
+        hipLaunchKernelGGL(k_group_count, dim3(nchunk), dim3(256), 0, st, d_ids, n, nexp, chunk, (int32_t *)d_work);
+    hipLaunchKernelGGL(k_group_place, dim3(nchunk), dim3(256), 0, st, d_ids, n, k, nexp, chunk,
                        nchunk > 1 ? (const int32_t *)d_work : nullptr, d_offsets, d_rows, d_slots);
     return hipGetLastError() == hipSuccess ? 0 : 4;
 }

@@ -20,14 +20,40 @@ struct RouteArgs {
     int sigmoid, renorm;
 };
 
+// the other lane of each pair at distance 1, 2, 4, 8 (within rows of 16 lanes, as a reduction needs it), 16 and 32
+template <int STEP> DEV float rt_other(float v) {
+    if (STEP >= 16) return __shfl_xor(v, STEP, 64);
+    constexpr int CTRL = STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x140;   // quads, half mirror, mirror
+    return ffrom((uint32_t)__builtin_amdgcn_mov_dpp((int)fbits(v), CTRL, 0xf, 0xf, true));
+}
 DEV float rt_max(float v) {     // over the wave, in every lane
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    v = fmaxf(v, rt_other<1>(v));
+    v = fmaxf(v, rt_other<2>(v));
+    v = fmaxf(v, rt_other<4>(v));
+    v = fmaxf(v, rt_other<8>(v));
+    v = fmaxf(v, rt_other<16>(v));
+    return fmaxf(v, rt_other<32>(v));
 }
 DEV float rt_sum(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+    v += rt_other<1>(v);
+    v += rt_other<2>(v);
+    v += rt_other<4>(v);
+    v += rt_other<8>(v);
+    v += rt_other<16>(v);
+    return v + rt_other<32>(v);
+}
+// a value that at least `count` lanes reach: the smallest of the maxima of as many groups of lanes
+DEV float rt_reached(float v, int count) {
+    const int g = count > 32 ? 1 : count > 16 ? 2 : count > 8 ? 4 : count > 4 ? 8 : count > 2 ? 16 : 32;   // lanes a group
+    float o;
+#define RT_STEP(S) o = rt_other<S>(v); v = S < g ? fmaxf(v, o) : fminf(v, o)
+    RT_STEP(1);
+    RT_STEP(2);
+    RT_STEP(4);
+    RT_STEP(8);
+    RT_STEP(16);
+    RT_STEP(32);
+#undef RT_STEP
     return v;
 }
 template <int SRC> DEV float rt_load(const void *p, int64_t i) {
@@ -38,52 +64,58 @@ template <int SRC> DEV float rt_load(const void *p, int64_t i) {
 
 #define RT_NONE (-__builtin_inff())
 
-// one wave a token; lane l holds experts l * P .. l * P + P - 1
+// One wave a token; lane l holds experts l, l + 64, ... The k largest keys are found in one pass: the smallest of the
+// maxima of at least k groups of lanes is reached by at least k keys, so only the keys that reach it (about three times
+// k) can be among them; they are moved to one a lane in index order and each counts the ones ahead of it. Where more than
+// 64 reach it, the largest is taken k times instead. A score is computed only where it is needed: logits order the
+// experts by themselves unless a bias or groups come in, and the sum over all cancels with renorm. Instructions bound
+// it: 16384 tokens of 384 experts take RT_TIME.
 template <int SRC, int P>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
-    __shared__ float keys[4][64 * P], gs[4][64];
+    __shared__ float keys[4][64 * P], gs[4][64], cand[4][64];
+    __shared__ int cid[4][64];
     const int lane = lane_id(), wave = threadIdx.x >> 6;
     const int64_t t = (int64_t)blockIdx.x * 4 + wave;
     const bool live = t < a.ntok;
     const int64_t row = (live ? t : a.ntok - 1) * a.ld;
-    float x[P], score[P], key[P];
+    float x[P], key[P];
     float mx = RT_NONE;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-        const int e = lane * P + j;
+        const int e = j * 64 + lane;
         float v = e < a.nexp ? rt_load<SRC>(a.logits, row + e) : RT_NONE;
         v = v == v ? fminf(v, 3.402823466e38f) : RT_NONE;
         x[j] = v;
         mx = fmaxf(mx, v);
     }
+    const bool by_logit = !a.bias && a.ngroup == 1;
     float z = 1.f;
-    if (a.sigmoid) {
-#pragma unroll
-        for (int j = 0; j < P; ++j) score[j] = 1.f / (1.f + expf(-x[j]));
-    } else {
+    if (!a.sigmoid) {
         mx = rt_max(mx);
-        float s = 0.f;
+        if (!by_logit || !a.renorm) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < P; ++j) s += x[j] == RT_NONE ? 0.f : expf(x[j] - mx);
+            z = rt_sum(s);
+            z = z > 0.f ? z : 1.f;
+        }
+    }
+    auto score = [&](float v) { return v == RT_NONE ? 0.f : a.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - mx) / z; };
+    if (by_logit) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) key[j] = x[j];
+    } else {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            score[j] = x[j] == RT_NONE ? 0.f : expf(x[j] - mx);
-            s += score[j];
+            const int e = j * 64 + lane;
+            float v = score(x[j]);
+            if (a.bias && e < a.nexp) v += a.bias[e];
+            key[j] = v == v && x[j] != RT_NONE ? v : RT_NONE;
         }
-        z = rt_sum(s);
-        z = z > 0.f ? z : 1.f;
-#pragma unroll
-        for (int j = 0; j < P; ++j) score[j] = score[j] / z;
-    }
-    const bool by_logit = !a.bias && a.ngroup == 1;
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-        const int e = lane * P + j;
-        float v = by_logit ? x[j] : score[j];
-        if (a.bias && e < a.nexp) v += a.bias[e];
-        key[j] = v == v && x[j] != RT_NONE ? v : RT_NONE;
     }
     if (a.ngroup > 1) {         // (uniform)
 #pragma unroll
-        for (int j = 0; j < P; ++j) keys[wave][lane * P + j] = key[j];
+        for (int j = 0; j < P; ++j) keys[wave][j * 64 + lane] = key[j];
         __syncthreads();
         const int per = a.nexp / a.ngroup;
         float best = RT_NONE, next = RT_NONE;
@@ -102,110 +134,138 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
         const uint64_t kept = __ballot(lane < a.ngroup && ahead < a.keep);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            const int e = lane * P + j;
+            const int e = j * 64 + lane;
             if (e < a.nexp && !((kept >> (e / per)) & 1)) key[j] = RT_NONE;
         }
     }
-    int my_id = -1;
-    float my_w = 0.f, sum = 0.f;
-    for (int r = 0; r < a.k; ++r) {
-        float v = key[0];
+    float top = key[0];
 #pragma unroll
-        for (int j = 1; j < P; ++j) v = fmaxf(v, key[j]);
-        const float m = rt_max(v);
-        if (m == RT_NONE) break;            // (uniform)
-        const int owner = __ffsll((unsigned long long)__ballot(v == m)) - 1;
-        int at = 0;
-        float s = 0.f;
-        bool found = false;
+    for (int j = 1; j < P; ++j) top = fmaxf(top, key[j]);
+    const float bound = rt_reached(top, a.k);
+    int n = 0;                  // the keys that reach it (none of minus infinity), in index order
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-            const bool hit = !found && key[j] == m;
-            at = hit ? j : at;
-            s = hit ? score[j] : s;
-            found |= hit;
-            if (hit && lane == owner) key[j] = RT_NONE;
+    for (int j = 0; j < P; ++j) {
+        const bool on = key[j] >= bound && key[j] != RT_NONE;
+        const uint64_t who = __ballot(on);
+        const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+        if (on && at < 64) {
+            cand[wave][at] = key[j];
+            cid[wave][at] = j * 64 + lane;
         }
-        s = __shfl(s, owner, 64);
-        at = __shfl(at, owner, 64);
-        sum += s;
-        if (lane == r) {
-            my_id = owner * P + at;
-            my_w = s;
+        n += __popcll(who);
+    }
+    __syncthreads();
+    int rank = 64, id = -1;     // this lane's candidate, if it is among the k
+    if (n <= 64) {
+        const float mine = lane < n ? cand[wave][lane] : RT_NONE;
+        id = lane < n ? cid[wave][lane] : -1;
+        int ahead = 0;
+        for (int i = 0; i < n; ++i) {
+            const float v = ffrom((uint32_t)__builtin_amdgcn_readlane((int)fbits(mine), i));
+            ahead += v > mine || (v == mine && i < lane);
+        }
+        if (lane < n && ahead < a.k) rank = ahead;
+    } else {
+        for (int r = 0; r < a.k; ++r) {                     // (n > 64 >= k: there is one every time)
+            float v = key[0];
+#pragma unroll
+            for (int j = 1; j < P; ++j) v = fmaxf(v, key[j]);
+            const float m = rt_max(v);
+            int best = -1;
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const uint64_t who = __ballot(key[j] == m);
+                if (best < 0 && who) best = j * 64 + __ffsll((unsigned long long)who) - 1;
+            }
+#pragma unroll
+            for (int j = 0; j < P; ++j)
+                if (j * 64 + lane == best) key[j] = RT_NONE;
+            if (lane == r) {
+                rank = r;
+                id = best;
+            }
         }
     }
+    __syncthreads();
+    if (lane < a.k) cid[wave][lane] = -1;
+    __syncthreads();
+    if (rank < a.k) cid[wave][rank] = id;
+    __syncthreads();
+    const int my_id = lane < a.k ? cid[wave][lane] : -1;
+    float my = 0.f;
+    if (my_id >= 0) {
+        float v = rt_load<SRC>(a.logits, row + my_id);
+        my = score(fminf(v, 3.402823466e38f));
+    }
+    float sum = 0.f;            // of the scores, best first
+    for (int r = 0; r < a.k; ++r) sum += ffrom((uint32_t)__builtin_amdgcn_readlane((int)fbits(my), r));
     if (live && lane < a.k) {
-        const float w = !a.renorm ? my_w : sum > 0.f ? my_w / sum : 0.f;
+        const float w = !a.renorm ? my : sum > 0.f ? my / sum : 0.f;
         a.ids[t * a.k + lane] = my_id;
         a.weights[t * a.k + lane] = w * a.scale;
     }
 }
 
-// ---- grouping: assignments (flat ids [n]) sorted by expert, in order within each. Chunks of RG_CHUNK assignments, a
-// workgroup each: counts per expert and chunk, then every chunk places its own from the counts of all.
-#define RG_CHUNK 2048
+// ---- grouping: assignments (flat ids [n]) sorted by expert, in order within each. Chunks of whole RG_BLOCKs (at most
+// RG_CHUNKS of them), a workgroup each: counts per chunk and expert, then every chunk places its own from the counts of all.
+#define RG_BLOCK 2048
+#define RG_CHUNKS 128
 #define RG_MAXE 1024
 
-// counts[e][chunk]
-__global__ __launch_bounds__(256) void k_group_count(const int32_t *__restrict__ ids, int64_t n, int nexp, int nchunk,
+// counts[chunk][e]
+__global__ __launch_bounds__(256) void k_group_count(const int32_t *__restrict__ ids, int64_t n, int nexp, int64_t chunk,
                                                      int32_t *__restrict__ counts) {
     __shared__ int hist[RG_MAXE];
     for (int e = threadIdx.x; e < nexp; e += 256) hist[e] = 0;
     __syncthreads();
-    const int64_t i0 = (int64_t)blockIdx.x * RG_CHUNK, i1 = i0 + RG_CHUNK < n ? i0 + RG_CHUNK : n;
+    const int64_t i0 = (int64_t)blockIdx.x * chunk, i1 = i0 + chunk < n ? i0 + chunk : n;
     for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
         const uint32_t e = (uint32_t)ids[i];
         if (e < (uint32_t)nexp) atomicAdd(&hist[e], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < nexp; e += 256) counts[(int64_t)e * nchunk + blockIdx.x] = hist[e];
+    for (int e = threadIdx.x; e < nexp; e += 256) counts[(int64_t)blockIdx.x * nexp + e] = hist[e];
 }
 
 // offsets [nexp + 1], rows [n] (the token of each sorted assignment), slots [n] (its flat index); the places past
-// offsets[nexp] (ids that name no expert) get -1. counts is null where there is one chunk.
+// offsets[nexp] (ids that name no expert) get -1. counts is null where there is one chunk. Each wave places a quarter of
+// the chunk, 64 assignments at a time: those of one expert find each other by the bits of its number, and the place of
+// each is the expert's next and the number of its own before it.
 __global__ __launch_bounds__(256) void k_group_place(const int32_t *__restrict__ ids, int64_t n, int k, int nexp,
-                                                     int nchunk, const int32_t *__restrict__ counts,
+                                                     int64_t chunk, const int32_t *__restrict__ counts,
                                                      int32_t *__restrict__ offsets, int32_t *__restrict__ rows,
                                                      int32_t *__restrict__ slots) {
     __shared__ int total[RG_MAXE], before[RG_MAXE], part[4], place[4][RG_MAXE];
-    const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, chunk = blockIdx.x;
-    const int64_t i0 = (int64_t)chunk * RG_CHUNK, i1 = i0 + RG_CHUNK < n ? i0 + RG_CHUNK : n;
-    for (int e = tid; e < 4 * RG_MAXE; e += 256) (&place[0][0])[e] = 0;
-    __syncthreads();
-    // each wave counts its own quarter of the chunk
-    const int64_t w0 = i0 + wave * (RG_CHUNK / 4);
-    int32_t id[RG_CHUNK / 256];
+    const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, me = blockIdx.x, nchunk = gridDim.x;
+    const int64_t i0 = me * chunk, i1 = i0 + chunk < n ? i0 + chunk : n, w0 = i0 + wave * (chunk / 4);
+    const int64_t w1 = w0 + chunk / 4 < i1 ? w0 + chunk / 4 : i1;
 #pragma unroll
-    for (int r = 0; r < RG_CHUNK / 256; ++r) {
-        const int64_t i = w0 + r * 64 + lane;
-        id[r] = i < i1 ? ids[i] : -1;
-        if ((uint32_t)id[r] < (uint32_t)nexp) atomicAdd(&place[wave][id[r]], 1);
-        else id[r] = -1;
+    for (int w = 0; w < 4; ++w)
+        for (int e = tid; e < nexp; e += 256) place[w][e] = 0;
+    __syncthreads();
+    for (int64_t i = w0 + lane; i < w1; i += 64) {
+        const uint32_t e = (uint32_t)ids[i];
+        if (e < (uint32_t)nexp) atomicAdd(&place[wave][e], 1);
+    }
+    // the whole call's totals and what earlier chunks hold
+    if (nchunk > 1) {
+        for (int e = tid; e < nexp; e += 256) {
+            int s = 0, b = 0;
+#pragma unroll 8
+            for (int c = 0; c < nchunk; ++c) {
+                const int v = counts[(int64_t)c * nexp + e];
+                s += v;
+                b += c < me ? v : 0;
+            }
+            total[e] = s;
+            before[e] = b;
+        }
     }
     __syncthreads();
-    // the whole call's totals and what earlier chunks hold
     if (nchunk == 1) {
         for (int e = tid; e < nexp; e += 256) {
             total[e] = place[0][e] + place[1][e] + place[2][e] + place[3][e];
             before[e] = 0;
-        }
-    } else {
-        for (int e = wave; e < nexp; e += 4) {
-            int s = 0, b = 0;
-            for (int c = lane; c < nchunk; c += 64) {
-                const int v = counts[(int64_t)e * nchunk + c];
-                s += v;
-                b += c < chunk ? v : 0;
-            }
-#pragma unroll
-            for (int o = 32; o; o >>= 1) {
-                s += __shfl_xor(s, o, 64);
-                b += __shfl_xor(b, o, 64);
-            }
-            if (lane == 0) {
-                total[e] = s;
-                before[e] = b;
-            }
         }
     }
     __syncthreads();
@@ -231,7 +291,7 @@ __global__ __launch_bounds__(256) void k_group_place(const int32_t *__restrict__
     for (int j = 0; j < 4; ++j) {
         const int e = 4 * tid + j;
         if (e < nexp) {
-            if (chunk == 0) offsets[e] = base;
+            if (me == 0) offsets[e] = base;
             int p = base + before[e];           // where each wave's first of this expert goes
             for (int w = 0; w < 4; ++w) {
                 const int c = place[w][e];
@@ -241,24 +301,24 @@ __global__ __launch_bounds__(256) void k_group_place(const int32_t *__restrict__
         }
         base += t[j];
     }
-    if (chunk == 0 && tid == 0) offsets[nexp] = all;
+    if (me == 0 && tid == 0) offsets[nexp] = all;
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < RG_CHUNK / 256; ++r) {
-        const int64_t i = w0 + r * 64 + lane;
-        const bool on = id[r] >= 0;
+    for (int64_t b = w0; b < w1; b += 64) {
+        const int64_t i = b + lane;
+        int id = i < w1 ? ids[i] : -1;
+        const bool on = (uint32_t)id < (uint32_t)nexp;
         uint64_t same = __ballot(on);
 #pragma unroll
-        for (int b = 0; b < 10; ++b) {
-            const uint64_t bit = __ballot((id[r] >> b) & 1);
-            same &= (id[r] >> b) & 1 ? bit : ~bit;
+        for (int j = 0; j < 10; ++j) {
+            const uint64_t bit = __ballot((id >> j) & 1);
+            same &= (id >> j) & 1 ? bit : ~bit;
         }
         if (on) {
             const int rank = __popcll(same & ((1ull << lane) - 1));
-            const int p = place[wave][id[r]] + rank;
+            const int p = place[wave][id] + rank;
             rows[p] = (int32_t)(i / k);
             slots[p] = (int32_t)i;
-            if (rank == 0) place[wave][id[r]] += __popcll(same);
+            if (rank == 0) place[wave][id] += __popcll(same);
         }
     }
     // (each chunk clears its share of what no expert took)

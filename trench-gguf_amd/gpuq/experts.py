@@ -8,6 +8,7 @@ on torch's current stream and returns without synchronizing, and raises ValueErr
 `gpuq/calibrate.py` runs them together.
 """
 from collections import namedtuple
+from functools import lru_cache
 
 import torch
 
@@ -25,8 +26,29 @@ Rows = namedtuple("Rows", "data n ncol")
 Group = namedtuple("Group", "offsets rows slots")
 
 
+# torch's current stream of a device as the C ABI takes it (the raw handle: a step's small calls feel a Stream object)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.device.index)
+
+
+# what the library says about sizes, asked once
+@lru_cache(maxsize=4096)
+def _bytes(gq, *sizes):
+    return gq.gpuq_mxfp4_bytes(*sizes)
+
+
+@lru_cache(maxsize=4096)
+def _work(gq, *sizes):
+    return gq.gpuq_mxfp4_matmul_work(*sizes)
+
+
+@lru_cache(maxsize=4096)
+def _group_work(gq, *sizes):
+    return gq.gpuq_route_group_work(*sizes)
 
 
 def _rows(x):
@@ -41,8 +63,8 @@ def _rows(x):
 
 def pack(gq, blocks, nmat, ne1, ne0):
     """ggml's MXFP4 blocks (uint8 on the device, nmat x ne1 rows of ne0 values) -> Packed, bit for bit"""
-    size = gq.gpuq_mxfp4_bytes(TILES, nmat, ne1, ne0)
-    want = gq.gpuq_mxfp4_bytes(BLOCKS, nmat, ne1, ne0)
+    size = _bytes(gq, TILES, nmat, ne1, ne0)
+    want = _bytes(gq, BLOCKS, nmat, ne1, ne0)
     if not size or blocks.dtype != torch.uint8 or not blocks.is_cuda or not blocks.is_contiguous() or \
             blocks.numel() != want:
         raise ValueError("expected %d contiguous bytes of MXFP4 blocks on the GPU" % want)
@@ -55,7 +77,7 @@ def pack(gq, blocks, nmat, ne1, ne0):
 
 def _quantize(gq, x, nmat, form, values):
     typ, ptr, n, ncol, ld = _rows(x)
-    size = gq.gpuq_mxfp4_bytes(form, nmat, n // nmat, ncol)
+    size = _bytes(gq, form, nmat, n // nmat, ncol)
     out = torch.empty(size, dtype=torch.uint8, device=x.device)
     back = torch.empty((n, ncol), dtype=torch.bfloat16, device=x.device) if values else None
     if not size or gq.gpuq_mxfp4_quantize_dev(typ, ptr, nmat, n // nmat, ncol, ld, form, out.data_ptr(),
@@ -114,11 +136,11 @@ def matmul(gq, x, w, group=None, up=None, out_dtype=torch.float32):
         if group.offsets.numel() != w.nmat + 1:
             raise ValueError("offsets must be one longer than the stack")
     y = torch.empty((m, w.ne1), dtype=out_dtype, device=dev)
-    size = gq.gpuq_mxfp4_matmul_work(typ, up is not None, n, w.nmat, w.ne1, w.ne0, group is not None, m)
+    size = _work(gq, typ, int(up is not None), n, w.nmat, w.ne1, w.ne0, int(group is not None), m)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     got = gq.gpuq_mxfp4_matmul_dev(typ, ptr, n, ld, w.data.data_ptr(), None if up is None else up.data.data_ptr(),
                                    w.nmat, w.ne1, w.ne0, offsets, rows, m, TYPES[out_dtype], y.data_ptr(),
-                                   work.data_ptr() if size else None, torch.cuda.current_stream(dev).cuda_stream)
+                                   work.data_ptr() if size else None, _raw_stream(dev.index))
     if not got:
         raise ValueError("gpuq_mxfp4_matmul_dev refused %d x %d rows and %d x %d x %d weights" %
                          (n, ncol, w.nmat, w.ne1, w.ne0))
@@ -150,8 +172,9 @@ def group(gq, ids, nexp):
     ptr = _index(ids, "ids")
     n, k = ids.shape
     offsets = torch.empty(nexp + 1, dtype=torch.int32, device=ids.device)
-    rows, slots = torch.empty((2, n * k), dtype=torch.int32, device=ids.device)
-    size = gq.gpuq_route_group_work(n * k, nexp)
+    rows = torch.empty(n * k, dtype=torch.int32, device=ids.device)
+    slots = torch.empty(n * k, dtype=torch.int32, device=ids.device)
+    size = _group_work(gq, n * k, nexp)
     work = torch.empty(size, dtype=torch.uint8, device=ids.device) if size else None
     rc = gq.gpuq_route_group_dev(ptr, n, k, nexp, offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
                                  work.data_ptr() if size else None, _stream(ids))
