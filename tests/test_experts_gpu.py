@@ -505,7 +505,8 @@ def test_route_with_nothing_left(gq, ex, score, with_bias):
 
 
 @pytest.mark.parametrize("n,k,nexp", [(1, 1, 1), (1, 8, 256), (3, 5, 7), (257, 8, 384), (2047, 1, 3), (1000, 6, 48),
-                                      (9000, 8, 1024), (4096, 2, 1)])
+                                      (9000, 8, 1024), (4096, 2, 1), (1023, 8, 40),
+                                      (1025, 8, 40), (150000, 8, 384)])
 def test_group(gq, ex, n, k, nexp):
     torch = torch_()
     rng = np.random.default_rng(n)
@@ -604,7 +605,7 @@ def test_refusals(gq, ex):
         assert r(*args) == 1, (at, bad)
     g = gq.gpuq_route_group_dev
     assert g(o, 0, 2, 8, o, o, o, None, st) == 1 and g(o, 4, 2, 2000, o, o, o, None, st) == 1
-    assert g(o, 4096, 2, 8, o, o, o, None, st) == 1             # needs scratch
+    assert g(o, 8192, 2, 8, o, o, o, None, st) == 1             # needs scratch
     w = ex.Packed(out, 1, 32, 480)
     for call in (lambda: ex.matmul(gq, x, w), lambda: ex.quantize(gq, x[:, :40]), lambda: ex.quantize(gq, x.t()),
                  lambda: ex.quantize(gq, x.cpu()), lambda: ex.route(gq, x, 3, score="other"),

@@ -275,6 +275,7 @@ extern "C" int gpuq_route_dev(int type, const void *d_logits, int64_t ntok, int6
 
 // assignments of a chunk: at most RG_CHUNKS chunks
 static int64_t group_chunk(int64_t n) {
+    if (n <= RG_SMALL) return RG_SMALL;
     return ((n + RG_BLOCK - 1) / RG_BLOCK + RG_CHUNKS - 1) / RG_CHUNKS * RG_BLOCK;
 }
 
@@ -294,8 +295,12 @@ extern "C" int gpuq_route_group_dev(const int32_t *d_ids, int64_t ntok, int k, i
     if (nchunk > 1 && !d_work) return 1;
     const hipStream_t st = (hipStream_t)stream;
     if (nchunk > 1)
-        hipLaunchKernelGGL(k_group_count, dim3(nchunk), dim3(256), 0, st, d_ids, n, nexp, chunk, (int32_t *)d_work);
-    hipLaunchKernelGGL(k_group_place, dim3(nchunk), dim3(256), 0, st, d_ids, n, k, nexp, chunk,
-                       nchunk > 1 ? (const int32_t *)d_work : nullptr, d_offsets, d_rows, d_slots);
+        hipLaunchKernelGGL(k_group_count, dim3(nchunk), dim3(1024), 0, st, d_ids, n, nexp, chunk, (int32_t *)d_work);
+    const int32_t *counts = nchunk > 1 ? (const int32_t *)d_work : nullptr;
+    if (n <= RG_SMALL)
+        hipLaunchKernelGGL(k_group_place<4>, dim3(1), dim3(256), 0, st, d_ids, n, k, nexp, chunk, counts, d_offsets, d_rows, d_slots);
+    else
+        hipLaunchKernelGGL(k_group_place<16>, dim3(nchunk), dim3(1024), 0, st, d_ids, n, k, nexp, chunk, counts, d_offsets, d_rows,
+                           d_slots);
     return hipGetLastError() == hipSuccess ? 0 : 4;
 }

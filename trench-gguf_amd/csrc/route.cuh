@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     if (a.ngroup > 1) {         // (uniform)
 #pragma unroll
         for (int j = 0; j < P; ++j) keys[wave][j * 64 + lane] = key[j];
-        __syncthreads();
+        __builtin_amdgcn_wave_barrier();
         const int per = a.nexp / a.ngroup;
         float best = RT_NONE, next = RT_NONE;
         if (lane < a.ngroup) {
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
         }
         const float g = next == RT_NONE ? best : best + next;
         gs[wave][lane] = g;
-        __syncthreads();
+        __builtin_amdgcn_wave_barrier();
         int ahead = 0;          // groups that come before this one
         for (int i = 0; i < a.ngroup; ++i) ahead += gs[wave][i] > g || (gs[wave][i] == g && i < lane);
         const uint64_t kept = __ballot(lane < a.ngroup && ahead < a.keep);
@@ -154,15 +154,18 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
         }
         n += __popcll(who);
     }
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();
     int rank = 64, id = -1;     // this lane's candidate, if it is among the k
     if (n <= 64) {
         const float mine = lane < n ? cand[wave][lane] : RT_NONE;
         id = lane < n ? cid[wave][lane] : -1;
         int ahead = 0;
-        for (int i = 0; i < n; ++i) {
-            const float v = ffrom((uint32_t)__builtin_amdgcn_readlane((int)fbits(mine), i));
-            ahead += v > mine || (v == mine && i < lane);
+        for (int i0 = 0; i0 < n; i0 += 8) {
+#pragma unroll
+            for (int i = i0; i < i0 + 8; ++i) {             // (lanes past n hold minus infinity)
+                const float v = ffrom((uint32_t)__builtin_amdgcn_readlane((int)fbits(mine), i));
+                ahead += v > mine || (v == mine && i < lane);
+            }
         }
         if (lane < n && ahead < a.k) rank = ahead;
     } else {
@@ -186,11 +189,11 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
             }
         }
     }
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();
     if (lane < a.k) cid[wave][lane] = -1;
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();
     if (rank < a.k) cid[wave][rank] = id;
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();
     const int my_id = lane < a.k ? cid[wave][lane] : -1;
     float my = 0.f;
     if (my_id >= 0) {
@@ -206,75 +209,94 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     }
 }
 
-// ---- grouping: assignments (flat ids [n]) sorted by expert, in order within each. Chunks of whole RG_BLOCKs (at most
-// RG_CHUNKS of them), a workgroup each: counts per chunk and expert, then every chunk places its own from the counts of all.
-#define RG_BLOCK 2048
+// ---- grouping: assignments (flat ids [n]) sorted by expert, in order within each. Chunks of 512 assignments a wave, a
+// workgroup each (of 16 waves, so that there are few: every chunk reads the counts of all; one of 4 where that holds the
+// whole call): counts per chunk and expert, then every chunk places its own.
+#define RG_SMALL 2048
+#define RG_BLOCK 8192
 #define RG_CHUNKS 128
 #define RG_MAXE 1024
 
+// the lanes of a wave find those with their number by its bits
+DEV uint64_t rg_same(int id, bool on) {
+    uint64_t same = __ballot(on);
+#pragma unroll
+    for (int j = 0; j < 10; ++j) {
+        const uint64_t bit = __ballot((id >> j) & 1);
+        same &= (id >> j) & 1 ? bit : ~bit;
+    }
+    return same;
+}
+
 // counts[chunk][e]
-__global__ __launch_bounds__(256) void k_group_count(const int32_t *__restrict__ ids, int64_t n, int nexp, int64_t chunk,
+__global__ __launch_bounds__(1024) void k_group_count(const int32_t *__restrict__ ids, int64_t n, int nexp, int64_t chunk,
                                                      int32_t *__restrict__ counts) {
     __shared__ int hist[RG_MAXE];
-    for (int e = threadIdx.x; e < nexp; e += 256) hist[e] = 0;
+    const int tid = threadIdx.x;
+    for (int e = tid; e < nexp; e += 1024) hist[e] = 0;
     __syncthreads();
     const int64_t i0 = (int64_t)blockIdx.x * chunk, i1 = i0 + chunk < n ? i0 + chunk : n;
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
-        const uint32_t e = (uint32_t)ids[i];
-        if (e < (uint32_t)nexp) atomicAdd(&hist[e], 1);
+    for (int64_t b = i0; b < i1; b += 8192) {
+        int32_t id[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) id[r] = b + r * 1024 + tid < i1 ? ids[b + r * 1024 + tid] : -1;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if ((uint32_t)id[r] < (uint32_t)nexp) atomicAdd(&hist[id[r]], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < nexp; e += 256) counts[(int64_t)blockIdx.x * nexp + e] = hist[e];
+    for (int e = tid; e < nexp; e += 1024) counts[(int64_t)blockIdx.x * nexp + e] = hist[e];
 }
 
 // offsets [nexp + 1], rows [n] (the token of each sorted assignment), slots [n] (its flat index); the places past
-// offsets[nexp] (ids that name no expert) get -1. counts is null where there is one chunk. Each wave places a quarter of
-// the chunk, 64 assignments at a time: those of one expert find each other by the bits of its number, and the place of
-// each is the expert's next and the number of its own before it.
-__global__ __launch_bounds__(256) void k_group_place(const int32_t *__restrict__ ids, int64_t n, int k, int nexp,
-                                                     int64_t chunk, const int32_t *__restrict__ counts,
-                                                     int32_t *__restrict__ offsets, int32_t *__restrict__ rows,
-                                                     int32_t *__restrict__ slots) {
-    __shared__ int total[RG_MAXE], before[RG_MAXE], part[4], place[4][RG_MAXE];
+// offsets[nexp] (ids that name no expert) get -1. counts is null where there is one chunk. Each of the NW waves places its
+// share of the chunk, 64 assignments at a time: the place of each is the expert's next and the number of its own before it.
+template <int NW>
+__global__ __launch_bounds__(NW * 64) void k_group_place(const int32_t *__restrict__ ids, int64_t n, int k, int nexp,
+                                                         int64_t chunk, const int32_t *__restrict__ counts,
+                                                         int32_t *__restrict__ offsets, int32_t *__restrict__ rows,
+                                                         int32_t *__restrict__ slots) {
+    constexpr int PER = RG_MAXE / (NW * 64);
+    __shared__ int part[NW], place[NW][RG_MAXE];
     const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, me = blockIdx.x, nchunk = gridDim.x;
-    const int64_t i0 = me * chunk, i1 = i0 + chunk < n ? i0 + chunk : n, w0 = i0 + wave * (chunk / 4);
-    const int64_t w1 = w0 + chunk / 4 < i1 ? w0 + chunk / 4 : i1;
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-        for (int e = tid; e < nexp; e += 256) place[w][e] = 0;
-    __syncthreads();
-    for (int64_t i = w0 + lane; i < w1; i += 64) {
-        const uint32_t e = (uint32_t)ids[i];
-        if (e < (uint32_t)nexp) atomicAdd(&place[wave][e], 1);
-    }
-    // the whole call's totals and what earlier chunks hold
+    const int64_t i0 = me * chunk, i1 = i0 + chunk < n ? i0 + chunk : n, w0 = i0 + wave * (chunk / NW);
+    const int64_t w1 = w0 + chunk / NW < i1 ? w0 + chunk / NW : i1;
+    // this thread's experts: the whole call's totals and what earlier chunks hold
+    int total[PER] = {}, before[PER] = {};
     if (nchunk > 1) {
-        for (int e = tid; e < nexp; e += 256) {
-            int s = 0, b = 0;
-#pragma unroll 8
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = PER * tid + j;
+            if (e >= nexp) continue;
+#pragma unroll 16
             for (int c = 0; c < nchunk; ++c) {
                 const int v = counts[(int64_t)c * nexp + e];
-                s += v;
-                b += c < me ? v : 0;
+                total[j] += v;
+                before[j] += c < me ? v : 0;
             }
-            total[e] = s;
-            before[e] = b;
         }
     }
-    __syncthreads();
-    if (nchunk == 1) {
-        for (int e = tid; e < nexp; e += 256) {
-            total[e] = place[0][e] + place[1][e] + place[2][e] + place[3][e];
-            before[e] = 0;
-        }
-    }
-    __syncthreads();
-    // exclusive scan of the totals: 4 experts a thread
-    int t[4], sum = 0;
+    for (int e = lane; e < nexp; e += 64) place[wave][e] = 0;
+    int32_t id[8];                              // 512 assignments at a time, the loads together
+    auto load = [&](int64_t b) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        t[j] = 4 * tid + j < nexp ? total[4 * tid + j] : 0;
-        sum += t[j];
+        for (int r = 0; r < 8; ++r) id[r] = b + r * 64 + lane < w1 ? ids[b + r * 64 + lane] : -1;
+    };
+    for (int64_t b = w0; b < w1; b += 512) {
+        load(b);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if ((uint32_t)id[r] < (uint32_t)nexp) atomicAdd(&place[wave][id[r]], 1);
+    }
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = PER * tid + j;
+        if (nchunk == 1 && e < nexp) {
+            for (int w = 0; w < NW; ++w) total[j] += place[w][e];
+        }
+        sum += total[j];
     }
     int inc = sum;
 #pragma unroll
@@ -284,45 +306,47 @@ __global__ __launch_bounds__(256) void k_group_place(const int32_t *__restrict__
     }
     if (lane == 63) part[wave] = inc;
     __syncthreads();
-    int base = inc - sum;
-    for (int w = 0; w < wave; ++w) base += part[w];
-    const int all = part[0] + part[1] + part[2] + part[3];
+    int base = inc - sum, all = 0;
+    for (int w = 0; w < NW; ++w) {
+        base += w < wave ? part[w] : 0;
+        all += part[w];
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int e = 4 * tid + j;
+    for (int j = 0; j < PER; ++j) {
+        const int e = PER * tid + j;
         if (e < nexp) {
             if (me == 0) offsets[e] = base;
-            int p = base + before[e];           // where each wave's first of this expert goes
-            for (int w = 0; w < 4; ++w) {
-                const int c = place[w][e];
+            int p = base + before[j], c[NW];    // where each wave's first of this expert goes
+#pragma unroll
+            for (int w = 0; w < NW; ++w) c[w] = place[w][e];
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
                 place[w][e] = p;
-                p += c;
+                p += c[w];
             }
         }
-        base += t[j];
+        base += total[j];
     }
     if (me == 0 && tid == 0) offsets[nexp] = all;
     __syncthreads();
-    for (int64_t b = w0; b < w1; b += 64) {
-        const int64_t i = b + lane;
-        int id = i < w1 ? ids[i] : -1;
-        const bool on = (uint32_t)id < (uint32_t)nexp;
-        uint64_t same = __ballot(on);
+    for (int64_t b = w0; b < w1; b += 512) {
+        if (w1 - w0 > 512) load(b);             // (otherwise they are still there)
 #pragma unroll
-        for (int j = 0; j < 10; ++j) {
-            const uint64_t bit = __ballot((id >> j) & 1);
-            same &= (id >> j) & 1 ? bit : ~bit;
-        }
-        if (on) {
-            const int rank = __popcll(same & ((1ull << lane) - 1));
-            const int p = place[wave][id] + rank;
-            rows[p] = (int32_t)(i / k);
-            slots[p] = (int32_t)i;
-            if (rank == 0) place[wave][id] += __popcll(same);
+        for (int r = 0; r < 8; ++r) {
+            const bool on = (uint32_t)id[r] < (uint32_t)nexp;
+            const uint64_t same = rg_same(id[r], on);
+            if (on) {
+                const uint32_t i = (uint32_t)(b + r * 64 + lane);
+                const int rank = __popcll(same & ((1ull << lane) - 1));
+                const int p = place[wave][id[r]] + rank;
+                rows[p] = (int32_t)(i / (uint32_t)k);
+                slots[p] = (int32_t)i;
+                if (rank == 0) place[wave][id[r]] += __popcll(same);
+            }
         }
     }
     // (each chunk clears its share of what no expert took)
-    for (int64_t i = i0 + tid; i < i1; i += 256) {
+    for (int64_t i = i0 + tid; i < i1; i += NW * 64) {
         if (i >= all) {
             rows[i] = -1;
             slots[i] = -1;
