@@ -22,7 +22,7 @@ def test_sizes(lib):
     assert lib.gpuq_mxfp4_matmul_work(30, 0, 8192, 1, 8192, 4096, 0, 8192) == 0
     assert [lib.gpuq_mxfp4_matmul_work(*a) for a in ((8, 0, 1, 1, 1, 32, 0, 1), (30, 0, 0, 1, 1, 32, 0, 1),
                                                      (0, 0, 1, 1, 1, 33, 0, 1), (0, 0, 1, 0, 1, 32, 0, 1))] == [0] * 4
-    assert lib.gpuq_route_group_work(8192, 64) == 0 and lib.gpuq_route_group_work(8193, 64) == 2 * 64 * 4
+    assert lib.gpuq_route_group_work(4096, 64) == 0 and lib.gpuq_route_group_work(4097, 64) == 2 * 64 * 4
     assert lib.gpuq_route_group_work(1 << 21, 64) == 128 * 64 * 4
 
 

@@ -27,10 +27,9 @@ int64_t stored_rows(int64_t nmat, int64_t nrow, int form) {
     return form == MX_TILES ? nmat * strips_of(nrow) * 16 : nmat * nrow;
 }
 
-template <int SRC> void launch_quantize(int form, const MxQuantArgs &p, hipStream_t st) {
-    const unsigned grid = (unsigned)((p.nblk + MX_U * 64 - 1) / (MX_U * 64));
-    if (form == MX_ROWS) hipLaunchKernelGGL((k_mx_quantize<SRC, MX_ROWS>), dim3(grid), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((k_mx_quantize<SRC, MX_BLOCKS>), dim3(grid), dim3(256), 0, st, p);
+template <int SRC> void launch_strips(bool tiles, dim3 grid, const MxQuantArgs &p, hipStream_t st) {
+    if (tiles) hipLaunchKernelGGL((k_mx_strips<SRC, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_mx_strips<SRC, false>), grid, dim3(256), 0, st, p);
 }
 
 int pieces_of(int x_type) { return x_type == T_F32 ? 3 : x_type == T_F16 ? 2 : 1; }
@@ -131,43 +130,40 @@ extern "C" size_t gpuq_mxfp4_quantize_dev(int src_type, const void *d_src, int64
     p.ld = ld;
     p.ncol = n_per_row;
     p.nb = (uint32_t)nb;
-    if (form == MX_TILES) {
-        const int64_t strips = strips_of(nrow);
+    if (form != MX_BLOCKS) {
+        const bool tiles = form == MX_TILES;
+        const int64_t per = strips_of(tiles ? nrow : rows), strips = tiles ? nmat * per : per;
         p.src = d_src;
-        p.nrow = nrow;
+        p.nrow = tiles ? nrow : rows;
         p.dst = (uint8_t *)d_dst;
-        p.scales = p.dst + nmat * strips * 8 * np;
+        p.scales = p.dst + (tiles ? strips * 16 : rows) * (np / 2);
         p.values = (uint16_t *)d_values;
-        p.row = mx_div((uint32_t)strips);
-        for (int64_t s = 0; s < nmat * strips; s += 65535) {
-            const dim3 grid((unsigned)(np / 512), (unsigned)std::min<int64_t>(65535, nmat * strips - s));
+        p.row = mx_div((uint32_t)per);
+        for (int64_t s = 0; s < strips; s += 65535) {
+            const dim3 grid((unsigned)(np / 512), (unsigned)std::min<int64_t>(65535, strips - s));
             p.row0 = s;
             switch (src_type) {
-                case T_F32: hipLaunchKernelGGL(k_mx_tiles<T_F32>, grid, dim3(256), 0, st, p); break;
-                case T_F16: hipLaunchKernelGGL(k_mx_tiles<T_F16>, grid, dim3(256), 0, st, p); break;
-                case T_BF16: hipLaunchKernelGGL(k_mx_tiles<T_BF16>, grid, dim3(256), 0, st, p); break;
-                default: hipLaunchKernelGGL(k_mx_tiles<T_MXFP4>, grid, dim3(256), 0, st, p);
+                case T_F32: launch_strips<T_F32>(tiles, grid, p, st); break;
+                case T_F16: launch_strips<T_F16>(tiles, grid, p, st); break;
+                case T_BF16: launch_strips<T_BF16>(tiles, grid, p, st); break;
+                default: launch_strips<T_MXFP4>(tiles, grid, p, st);
             }
             if (hipGetLastError() != hipSuccess) return 0;
         }
         return size;
     }
-    const int64_t stored = form == MX_ROWS ? np / 32 : nb, rows_max = MAX_BLOCKS / stored;
-    p.nrow = rows;
-    p.row = mx_div((uint32_t)stored);
-    p.scales = form == MX_ROWS ? (uint8_t *)d_dst + rows * stored * 16 : nullptr;
+    const int64_t rows_max = MAX_BLOCKS / nb;
+    p.row = mx_div((uint32_t)nb);
     for (int64_t r = 0; r < rows; r += rows_max) {
-        p.src = (const uint8_t *)d_src + (src_type == T_MXFP4 ? r * nb * 17 : r * ld * type_size(src_type));
-        p.dst = (uint8_t *)d_dst + r * stored * (form == MX_ROWS ? 16 : 17);
+        p.src = (const uint8_t *)d_src + r * ld * type_size(src_type);
+        p.dst = (uint8_t *)d_dst + r * nb * 17;
         p.values = d_values ? (uint16_t *)d_values + r * n_per_row : nullptr;
-        p.row0 = r;
-        p.nblk = (uint32_t)(std::min(rows_max, rows - r) * stored);
+        p.nblk = (uint32_t)(std::min(rows_max, rows - r) * nb);
+        const dim3 grid((p.nblk + MX_U * 64 - 1) / (MX_U * 64));
         switch (src_type) {
-            case T_F32: launch_quantize<T_F32>(form, p, st); break;
-            case T_F16: launch_quantize<T_F16>(form, p, st); break;
-            case T_BF16: launch_quantize<T_BF16>(form, p, st); break;
-            default: hipLaunchKernelGGL((k_mx_quantize<T_MXFP4, MX_ROWS>), dim3((p.nblk + MX_U * 64 - 1) / (MX_U * 64)),
-                                        dim3(256), 0, st, p);
+            case T_F32: hipLaunchKernelGGL(k_mx_blocks<T_F32>, grid, dim3(256), 0, st, p); break;
+            case T_F16: hipLaunchKernelGGL(k_mx_blocks<T_F16>, grid, dim3(256), 0, st, p); break;
+            default: hipLaunchKernelGGL(k_mx_blocks<T_BF16>, grid, dim3(256), 0, st, p);
         }
         if (hipGetLastError() != hipSuccess) return 0;
     }
@@ -300,7 +296,7 @@ extern "C" int gpuq_route_group_dev(const int32_t *d_ids, int64_t ntok, int k, i
     if (n <= RG_SMALL)
         hipLaunchKernelGGL(k_group_place<4>, dim3(1), dim3(256), 0, st, d_ids, n, k, nexp, chunk, counts, d_offsets, d_rows, d_slots);
     else
-        hipLaunchKernelGGL(k_group_place<16>, dim3(nchunk), dim3(1024), 0, st, d_ids, n, k, nexp, chunk, counts, d_offsets, d_rows,
+        hipLaunchKernelGGL(k_group_place<8>, dim3(nchunk), dim3(512), 0, st, d_ids, n, k, nexp, chunk, counts, d_offsets, d_rows,
                            d_slots);
     return hipGetLastError() == hipSuccess ? 0 : 4;
 }

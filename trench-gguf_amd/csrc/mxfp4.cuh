@@ -99,10 +99,10 @@ struct MxQuantArgs {
     int64_t ld;                 // source elements from row to row (MXFP4: unused, rows are whole blocks)
     uint8_t *dst, *scales;      // blocks, or codes and scales
     uint16_t *values;           // BF16, or null
-    int64_t ncol, nrow;         // of the whole call (rows), of a matrix (tiles)
-    int64_t row0;               // the launch's first row (rows)
-    uint32_t nblk, nb;          // blocks of this launch, and those of a row that hold values
-    MxDiv row;                  // blocks of a row as stored (nb, or with the padding); tiles: strips of a matrix
+    int64_t ncol, nrow;         // columns, and rows of a matrix (rows: of all of them together)
+    int64_t row0;               // the launch's first strip
+    uint32_t nblk, nb;          // blocks of this launch (blocks), and those of a row
+    MxDiv row;                  // blocks of a row (blocks), strips of a matrix
 };
 
 enum { MX_BLOCKS = 0, MX_ROWS = 1, MX_TILES = 2 };
@@ -145,73 +145,68 @@ template <int SRC> DEV uint32_t mx_encode(int a, const float (&v)[8], const uint
     return codes;
 }
 
-// blocks and rows: four lanes a block, 8 values a lane, MX_U blocks a lane
+// blocks: four lanes a block, 8 values a lane, MX_U blocks a lane; the 17-byte blocks of a workgroup leave through LDS
 #define MX_U 4
-template <int SRC, int FORM>
-__global__ __launch_bounds__(256) void k_mx_quantize(MxQuantArgs p) {
-    __shared__ __align__(16) uint8_t out[FORM == MX_ROWS ? 16 : MX_U * 64 * 17];
+template <int SRC>
+__global__ __launch_bounds__(256) void k_mx_blocks(MxQuantArgs p) {
+    __shared__ __align__(16) uint8_t out[MX_U * 64 * 17];
     const int tid = threadIdx.x, a = tid & 3;
     const uint32_t b0 = blockIdx.x * (MX_U * 64) + (tid >> 2);
     float v[MX_U][8];
-    uint32_t raw[MX_U][3], row[MX_U], col[MX_U];
+    uint32_t raw[3], row[MX_U], col[MX_U];
 #pragma unroll
     for (int u = 0; u < MX_U; ++u) {
         const uint32_t b = b0 + 64 * u < p.nblk ? b0 + 64 * u : p.nblk - 1;
         row[u] = p.row.div(b);
         col[u] = b - row[u] * p.row.d;
-        mx_source<SRC>(p, row[u], col[u], col[u] < p.nb, a, v[u], raw[u]);
+        mx_source<SRC>(p, row[u], col[u], true, a, v[u], raw);
     }
 #pragma unroll
     for (int u = 0; u < MX_U; ++u) {
-        const bool in = b0 + 64 * u < p.nblk;
         uint32_t e;
-        const uint32_t codes = mx_encode<SRC>(a, v[u], raw[u], e), c = col[u];
-        if (p.values && in && c < p.nb)
-            *(uint4 *)(p.values + (int64_t)row[u] * p.ncol + c * 32 + 8 * a) = mx_values(codes, e);
-        if (FORM == MX_ROWS) {
-            if (in) *(uint32_t *)(p.dst + ((int64_t)row[u] * p.row.d + c) * 16 + 4 * a) = codes;
-            if (in && a == 0)
-                p.scales[((int64_t)(c >> 4) * p.nrow + p.row0 + row[u]) * 16 + 4 * (c & 3) + ((c >> 2) & 3)] = (uint8_t)e;
-        } else {
-            // ggml's block: e, then byte j = value j | value j + 16 << 4; lane a gets bytes 4a .. 4a + 3
-            const uint32_t lo = mx_quad<0x50>(codes) >> (16 * (a & 1)), hi = mx_quad<0xFA>(codes) >> (16 * (a & 1));
-            const uint32_t w = mx_spread(lo & 0xffffu) | (mx_spread(hi & 0xffffu) << 4);
-            uint8_t *o = out + (u * 64 + (tid >> 2)) * 17;
-            if (a == 0) o[0] = (uint8_t)e;
+        const uint32_t codes = mx_encode<SRC>(a, v[u], raw, e);
+        if (p.values && b0 + 64 * u < p.nblk)
+            *(uint4 *)(p.values + (int64_t)row[u] * p.ncol + col[u] * 32 + 8 * a) = mx_values(codes, e);
+        // ggml's block: e, then byte j = value j | value j + 16 << 4; lane a gets bytes 4a .. 4a + 3
+        const uint32_t lo = mx_quad<0x50>(codes) >> (16 * (a & 1)), hi = mx_quad<0xFA>(codes) >> (16 * (a & 1));
+        const uint32_t w = mx_spread(lo & 0xffffu) | (mx_spread(hi & 0xffffu) << 4);
+        uint8_t *o = out + (u * 64 + (tid >> 2)) * 17;
+        if (a == 0) o[0] = (uint8_t)e;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[1 + 4 * a + j] = (uint8_t)(w >> (8 * j));
-        }
+        for (int j = 0; j < 4; ++j) o[1 + 4 * a + j] = (uint8_t)(w >> (8 * j));
     }
-    if (FORM == MX_BLOCKS) {
-        __syncthreads();
-        const uint32_t first = blockIdx.x * (MX_U * 64);
-        const uint32_t n = (p.nblk - first < MX_U * 64 ? p.nblk - first : MX_U * 64) * 17;
-        uint8_t *d = p.dst + (int64_t)first * 17;
-        for (uint32_t i = tid * 16; i < n; i += 256 * 16) {
-            if (i + 16 <= n) {
-                *(uint4 *)(d + i) = *(const uint4 *)(out + i);
-            } else {
-                for (uint32_t j = i; j < n; ++j) d[j] = out[j];
-            }
+    __syncthreads();
+    const uint32_t first = blockIdx.x * (MX_U * 64);
+    const uint32_t n = (p.nblk - first < MX_U * 64 ? p.nblk - first : MX_U * 64) * 17;
+    uint8_t *d = p.dst + (int64_t)first * 17;
+    for (uint32_t i = tid * 16; i < n; i += 256 * 16) {
+        if (i + 16 <= n) {
+            *(uint4 *)(d + i) = *(const uint4 *)(out + i);
+        } else {
+            for (uint32_t j = i; j < n; ++j) d[j] = out[j];
         }
     }
 }
 
-// tiles: a workgroup writes a strip's 512 columns, four pieces of 128; grid (np / 512, strips of the launch)
-template <int SRC>
-__global__ __launch_bounds__(256) void k_mx_tiles(MxQuantArgs p) {
+// rows and tiles: a workgroup writes 512 columns of 16 rows, four pieces of 128; grid (np / 512, strips of the launch).
+// (Rows made block by block, a row's scales of 512 columns apart from the next row's in time and place, took 46 us of
+// 8192 x 7168 BF16 values, and MX_ROWS_US so: 16 rows' scales are two whole lines.)
+template <int SRC, bool TILES>
+__global__ __launch_bounds__(256) void k_mx_strips(MxQuantArgs p) {
     __shared__ uint32_t es[64];
     const int tid = threadIdx.x, a = tid & 3, q = (tid >> 2) & 3, r = tid >> 4;
     const uint32_t strip = (uint32_t)p.row0 + blockIdx.y, mat = p.row.div(strip);
     const int64_t in_mat = (int64_t)(strip - mat * p.row.d) * 16 + r, row = mat * p.nrow + in_mat;
+    const bool has = in_mat < p.nrow;
     float v[4][8];
     uint32_t raw[4][3];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const uint32_t col = blockIdx.x * 16 + 4 * c + q;
-        mx_source<SRC>(p, row, col, in_mat < p.nrow && col < p.nb, a, v[c], raw[c]);
+        mx_source<SRC>(p, row, col, has && col < p.nb, a, v[c], raw[c]);
     }
-    uint8_t *d = p.dst + ((int64_t)strip * gridDim.x + blockIdx.x) * 4096;
+    uint8_t *d = TILES ? p.dst + ((int64_t)strip * gridDim.x + blockIdx.x) * 4096 + (16 * q + r) * 16 + 4 * a
+                       : p.dst + (row * gridDim.x + blockIdx.x) * 256 + 16 * q + 4 * a;
     uint32_t all = 0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -219,13 +214,17 @@ __global__ __launch_bounds__(256) void k_mx_tiles(MxQuantArgs p) {
         uint32_t e;
         const uint32_t codes = mx_encode<SRC>(a, v[c], raw[c], e);
         all |= e << (8 * c);
-        *(uint32_t *)(d + c * 1024 + (16 * q + r) * 16 + 4 * a) = codes;
-        if (p.values && in_mat < p.nrow && col < p.nb)
+        if (TILES || has) *(uint32_t *)(d + c * (TILES ? 1024 : 64)) = codes;
+        if (p.values && has && col < p.nb)
             *(uint4 *)(p.values + row * p.ncol + col * 32 + 8 * a) = mx_values(codes, e);
     }
-    if (a == 0) es[16 * q + r] = all;
+    if (a == 0) es[TILES ? 16 * q + r : 4 * r + q] = all;
     __syncthreads();
-    if (tid < 64) *(uint32_t *)(p.scales + ((int64_t)strip * gridDim.x + blockIdx.x) * 256 + 4 * tid) = es[tid];
+    if (TILES) {
+        if (tid < 64) *(uint32_t *)(p.scales + ((int64_t)strip * gridDim.x + blockIdx.x) * 256 + 4 * tid) = es[tid];
+    } else if (tid < 64 && (int64_t)strip * 16 + (tid >> 2) < p.nrow) {       // (rows: one matrix of them all)
+        *(uint32_t *)(p.scales + ((int64_t)blockIdx.x * p.nrow + (int64_t)strip * 16) * 16 + 4 * tid) = es[tid];
+    }
 }
 
 // F32 / F16 rows as sums of BF16 rows: the top 16 bits, then those of the rest, which holds every bit of an F16 value

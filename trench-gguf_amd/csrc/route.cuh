@@ -72,9 +72,10 @@ template <int SRC> DEV float rt_load(const void *p, int64_t i) {
 // it: 16384 tokens of 384 experts take RT_TIME.
 template <int SRC, int P>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
-    __shared__ float keys[4][64 * P], gs[4][64], cand[4][64];
+    __shared__ float keys[4][64 * P], gs[4][64];
+    __shared__ int2 cand[4][64];                            // (key, expert)
     __shared__ int cid[4][64];
-    const int lane = lane_id(), wave = threadIdx.x >> 6;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t t = (int64_t)blockIdx.x * 4 + wave;
     const bool live = t < a.ntok;
     const int64_t row = (live ? t : a.ntok - 1) * a.ld;
@@ -148,24 +149,22 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
         const bool on = key[j] >= bound && key[j] != RT_NONE;
         const uint64_t who = __ballot(on);
         const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-        if (on && at < 64) {
-            cand[wave][at] = key[j];
-            cid[wave][at] = j * 64 + lane;
-        }
+        if (on && at < 64) cand[wave][at] = make_int2((int)fbits(key[j]), j * 64 + lane);
         n += __popcll(who);
     }
     __builtin_amdgcn_wave_barrier();
     int rank = 64, id = -1;     // this lane's candidate, if it is among the k
     if (n <= 64) {
-        const float mine = lane < n ? cand[wave][lane] : RT_NONE;
-        id = lane < n ? cid[wave][lane] : -1;
+        // keys as whole numbers in the same order: one from before this lane is ahead if it is not less, one from behind if
+        // it is more (lanes past n hold less than all)
+        const int2 c = cand[wave][lane];
+        const int b = c.x == (int)0x80000000 ? 0 : c.x;     // (minus zero ties with zero)
+        const int mine = lane < n ? (b < 0 ? b ^ 0x7fffffff : b) : (int)0x80000000;
+        id = lane < n ? c.y : -1;
         int ahead = 0;
         for (int i0 = 0; i0 < n; i0 += 8) {
 #pragma unroll
-            for (int i = i0; i < i0 + 8; ++i) {             // (lanes past n hold minus infinity)
-                const float v = ffrom((uint32_t)__builtin_amdgcn_readlane((int)fbits(mine), i));
-                ahead += v > mine || (v == mine && i < lane);
-            }
+            for (int i = i0; i < i0 + 8; ++i) ahead += __builtin_amdgcn_readlane(mine, i) > (i < lane ? mine - 1 : mine);
         }
         if (lane < n && ahead < a.k) rank = ahead;
     } else {
@@ -210,10 +209,10 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
 }
 
 // ---- grouping: assignments (flat ids [n]) sorted by expert, in order within each. Chunks of 512 assignments a wave, a
-// workgroup each (of 16 waves, so that there are few: every chunk reads the counts of all; one of 4 where that holds the
-// whole call): counts per chunk and expert, then every chunk places its own.
+// workgroup each (of 8 waves: every chunk reads the counts of all, so few are better, and many share the work; one of 4 where
+// that holds the whole call): counts per chunk and expert, then every chunk places its own.
 #define RG_SMALL 2048
-#define RG_BLOCK 8192
+#define RG_BLOCK 4096
 #define RG_CHUNKS 128
 #define RG_MAXE 1024
 
