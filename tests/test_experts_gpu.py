@@ -193,6 +193,33 @@ def test_quantize_takes_strided_rows_and_many_blocks(gq, ex, src):
     assert bool((out[size:] == 0xA5).all())
 
 
+@pytest.mark.parametrize("src", ["f16", "bf16"])
+def test_quantize_every_16_bit_value(gq, ex, src):
+    """every finite pattern, in blocks whose largest value puts the scale at 2^0, 2^-2 and 2^-9"""
+    torch = torch_()
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16)
+    v = bits.view(dtype(src)).float()
+    for top in (4.0, 1.75, 0.0078125):
+        x = torch.where(torch.isfinite(v) & (v.abs() <= top), v, 0.0)
+        x = torch.cat((torch.full((len(x) // 31 + 1, 1), top), torch.nn.functional.pad(x, (0, 31 - len(x) % 31)).view(-1, 31)), 1)
+        x = x.to(dtype(src))
+        code, e = round_blocks(x.double().numpy())
+        assert np.array_equal(ex.quantize_blocks(gq, x.cuda()).cpu().numpy(), as_blocks(code, e))
+
+
+def test_quantize_beside_every_tie(gq, ex):
+    """F32 values at, a unit above and a unit below each tie and level, at several scales"""
+    torch = torch_()
+    mid = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=np.float32)
+    v = np.concatenate([s * np.concatenate((mid, np.nextafter(mid, np.float32(9)), np.nextafter(mid, np.float32(0))))
+                        for s in (np.float32(1), np.float32(-1))])
+    v = np.pad(v, (0, 93 - len(v))).reshape(3, 31)
+    rows = np.concatenate([np.concatenate((np.full((3, 1), 7.5, np.float32), v), axis=1) * np.float32(2.0 ** k)
+                           for k in (0, -6, 20, -120, 120)])
+    code, e = round_blocks(rows.astype(np.float64))
+    assert np.array_equal(ex.quantize_blocks(gq, torch.from_numpy(rows).cuda()).cpu().numpy(), as_blocks(code, e))
+
+
 def test_quantize_of_nan_and_infinity(gq, ex):
     torch = torch_()
     x = torch.zeros(4, 64)

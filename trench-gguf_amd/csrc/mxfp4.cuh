@@ -52,35 +52,83 @@ DEV uint32_t mx_gather(uint32_t b) {
     return (b | (b >> 8)) & 0xffffu;
 }
 
-// 8 source values
-template <int SRC> DEV void mx_load8(const void *src, int64_t i, float (&v)[8]) {
-    if (SRC == T_F32) {
-        const float4 a = *(const float4 *)((const float *)src + i), b = *(const float4 *)((const float *)src + i + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 a = *(const uint4 *)((const uint16_t *)src + i);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 8 source values as they are stored
+template <int SRC> struct MxRaw { uint32_t w[SRC == T_F32 ? 8 : 4]; };
+template <int SRC> DEV MxRaw<SRC> mx_load8(const void *src, int64_t i) {
+    MxRaw<SRC> r;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (SRC == T_BF16) {
-                v[2 * j] = ffrom(w[j] << 16);
-                v[2 * j + 1] = ffrom(w[j] & 0xffff0000u);
-            } else {
-                union { uint32_t u; _Float16 h[2]; } c = {w[j]};
-                v[2 * j] = (float)c.h[0];
-                v[2 * j + 1] = (float)c.h[1];
-            }
+    for (int k = 0; k < (SRC == T_F32 ? 2 : 1); ++k) {
+        const uint4 a = *((const uint4 *)((const uint8_t *)src + i * (SRC == T_F32 ? 4 : 2)) + k);
+        r.w[4 * k] = a.x;
+        r.w[4 * k + 1] = a.y;
+        r.w[4 * k + 2] = a.z;
+        r.w[4 * k + 3] = a.w;
+    }
+    return r;
+}
+template <int SRC> DEV void mx_float8(const MxRaw<SRC> &r, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (SRC == T_F32) {
+            v[j] = ffrom(r.w[j % (SRC == T_F32 ? 8 : 4)]);
+        } else if (SRC == T_BF16) {
+            v[j] = ffrom(j & 1 ? r.w[j / 2] & 0xffff0000u : r.w[j / 2] << 16);
+        } else {
+            union { uint32_t u; _Float16 h[2]; } c = {r.w[j / 2]};
+            v[j] = (float)c.h[j & 1];
         }
     }
 }
 
-// the code of v at the scale whose reciprocal is inv
-DEV uint32_t mx_code(float v, float inv) {
-    const float t = fabsf(v) * inv;
-    const uint32_t c = (uint32_t)(t > 0.25f) + (t > 0.75f) + (t > 1.25f) + (t > 1.75f) + (t > 2.5f) + (t > 3.5f) +
-                       (t > 5.f);
-    return c ? c | ((fbits(v) >> 28) & 8u) : 0u;
+typedef unsigned short mx_u2 __attribute__((ext_vector_type(2)));
+// the largest magnitude of the 8 as f32 and whether they are all finite: magnitudes order as their bits do, two halves at
+// a time
+template <int SRC> DEV float mx_largest(const MxRaw<SRC> &r, bool &finite) {
+    if (SRC == T_F32) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t b = r.w[j % (SRC == T_F32 ? 8 : 4)] & 0x7fffffffu;
+            m = b > m ? b : m;
+        }
+        finite = m < 0x7f800000u;
+        return ffrom(m);
+    }
+    union { uint32_t u; mx_u2 h; } m = {0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        union { uint32_t u; mx_u2 h; } b = {r.w[j] & 0x7fff7fffu};
+        m.h = __builtin_elementwise_max(m.h, b.h);
+    }
+    const uint32_t top = (m.u >> 16) > (m.u & 0xffffu) ? m.u >> 16 : m.u & 0xffffu;
+    finite = top < (SRC == T_BF16 ? 0x7f80u : 0x7c00u);
+    if (SRC == T_BF16) return ffrom(top << 16);
+    union { uint16_t u; _Float16 h; } c = {(uint16_t)top};
+    return (float)c.h;
+}
+
+// The codes of 8 values at the scale 2^(e - 127). The conversion rounds to nearest even; a tie is to go to the smaller
+// magnitude, so what it gets is the next number below (a power of two less one unit is the factor that gives it). Of 16-bit
+// sources that moves no other value over a tie, since none lies within a unit of f32 above one; of F32 values only those
+// with two bits after the first, every tie among them, are moved. (Seven comparisons a value took three times the
+// instructions, and they bound the rounding: 8192 x 7168 BF16 values 43 us, with the conversion 24.) No negative zero.
+template <int SRC> DEV uint32_t mx_codes(const float (&v)[8], uint32_t e) {
+    const float inv = ffrom((254 - e) << 23), below = ffrom(((254 - e) << 23) - 1);
+    float t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        t[j] = v[j] * below;
+        if (SRC == T_F32) {
+            const float u = v[j] * inv;
+            t[j] = fbits(u) & 0x1fffffu ? u : t[j];
+        }
+    }
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, t[0], t[1], 1.f, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, t[2], t[3], 1.f, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, t[4], t[5], 1.f, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, t[6], t[7], 1.f, 3);
+    return c & (((c & 0x77777777u) + 0x77777777u) | 0x77777777u);
 }
 
 // 8 codes and their block's scale exponent -> 8 BF16 values (exact: a value is at least 2^-128)
@@ -107,42 +155,46 @@ struct MxQuantArgs {
 
 enum { MX_BLOCKS = 0, MX_ROWS = 1, MX_TILES = 2 };
 
-// 8 values of a block (quarter a of it): the source's, zero where the block holds none
-template <int SRC> DEV void mx_source(const MxQuantArgs &p, int64_t row, uint32_t col, bool real, int a, float (&v)[8],
-                                      uint32_t (&raw)[3]) {
-    if (SRC == T_MXFP4) {
+// quarter a of a block as the source has it, zero where it holds none: 8 values, or of MXFP4 8 bytes of codes and the scale
+template <int SRC> struct MxQuarter { MxRaw<SRC == T_MXFP4 ? T_BF16 : SRC> r; };
+template <int SRC> DEV MxQuarter<SRC> mx_source(const MxQuantArgs &p, int64_t row, uint32_t col, bool real, int a) {
+    MxQuarter<SRC> v;
+    if constexpr (SRC == T_MXFP4) {
         const uint8_t *blk = (const uint8_t *)p.src + (real ? row * p.nb + col : 0) * 17;
-        raw[2] = blk[0];
-        __builtin_memcpy(&raw[0], blk + 1 + 8 * (a & 1), 8);
-        if (!real) raw[0] = raw[1] = raw[2] = 0;
+        v.r.w[2] = blk[0];
+        __builtin_memcpy(&v.r.w[0], blk + 1 + 8 * (a & 1), 8);
     } else {
-        mx_load8<SRC>(p.src, (real ? row * p.ld + (int64_t)col * 32 : 0) + 8 * a, v);
-        if (!real) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        }
+        v.r = mx_load8<SRC>(p.src, (real ? row * p.ld + (int64_t)col * 32 : 0) + 8 * a);
     }
-}
-// their codes and the block's scale exponent (over the 4 lanes that share it)
-template <int SRC> DEV uint32_t mx_encode(int a, const float (&v)[8], const uint32_t (&raw)[3], uint32_t &e) {
-    uint32_t codes = 0;
-    if (SRC == T_MXFP4) {
-        const int sh = 4 * (a >> 1);
-        codes = mx_gather((raw[0] >> sh) & 0x0f0f0f0fu) | (mx_gather((raw[1] >> sh) & 0x0f0f0f0fu) << 16);
-        e = raw[2];
-    } else {
-        float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));             // (a NaN is passed over)
+    for (int j = 0; j < (SRC == T_F32 ? 8 : SRC == T_MXFP4 ? 3 : 4); ++j) v.r.w[j] = real ? v.r.w[j] : 0;
+    return v;
+}
+// its codes and the block's scale exponent (over the 4 lanes that share it; every lane of the wave takes part)
+template <int SRC> DEV uint32_t mx_encode(int a, const MxQuarter<SRC> &q, uint32_t &e) {
+    if constexpr (SRC == T_MXFP4) {
+        const int sh = 4 * (a >> 1);
+        e = q.r.w[2];
+        return mx_gather((q.r.w[0] >> sh) & 0x0f0f0f0fu) | (mx_gather((q.r.w[1] >> sh) & 0x0f0f0f0fu) << 16);
+    } else {
+        float v[8];
+        bool finite;
+        mx_float8<SRC>(q.r, v);
+        float m = mx_largest<SRC>(q.r, finite);
+        if (__builtin_expect(__any(!finite), 0)) {          // NaN as zero, infinities as the largest
+            m = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = v[j] == v[j] ? fminf(fmaxf(v[j], -3.402823466e38f), 3.402823466e38f) : 0.f;
+                m = fmaxf(m, fabsf(v[j]));
+            }
+        }
         m = fmaxf(m, ffrom(mx_quad<0xB1>(fbits(m))));
         m = fmaxf(m, ffrom(mx_quad<0x4E>(fbits(m))));
-        const int x = (int)(fbits(m) >> 23) - 2;
-        e = (uint32_t)(x < 0 ? 0 : x > 252 ? 252 : x);
-        const float inv = ffrom((254 - e) << 23);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) codes |= mx_code(v[j], inv) << (4 * j);
+        const int x = (int)(fbits(m) >> 23) - 2;            // (at most 252)
+        e = (uint32_t)(x < 0 ? 0 : x);
+        return mx_codes<SRC>(v, e);
     }
-    return codes;
 }
 
 // blocks: four lanes a block, 8 values a lane, MX_U blocks a lane; the 17-byte blocks of a workgroup leave through LDS
@@ -152,19 +204,19 @@ __global__ __launch_bounds__(256) void k_mx_blocks(MxQuantArgs p) {
     __shared__ __align__(16) uint8_t out[MX_U * 64 * 17];
     const int tid = threadIdx.x, a = tid & 3;
     const uint32_t b0 = blockIdx.x * (MX_U * 64) + (tid >> 2);
-    float v[MX_U][8];
-    uint32_t raw[3], row[MX_U], col[MX_U];
+    MxQuarter<SRC> v[MX_U];
+    uint32_t row[MX_U], col[MX_U];
 #pragma unroll
     for (int u = 0; u < MX_U; ++u) {
         const uint32_t b = b0 + 64 * u < p.nblk ? b0 + 64 * u : p.nblk - 1;
         row[u] = p.row.div(b);
         col[u] = b - row[u] * p.row.d;
-        mx_source<SRC>(p, row[u], col[u], true, a, v[u], raw);
+        v[u] = mx_source<SRC>(p, row[u], col[u], true, a);
     }
 #pragma unroll
     for (int u = 0; u < MX_U; ++u) {
         uint32_t e;
-        const uint32_t codes = mx_encode<SRC>(a, v[u], raw, e);
+        const uint32_t codes = mx_encode<SRC>(a, v[u], e);
         if (p.values && b0 + 64 * u < p.nblk)
             *(uint4 *)(p.values + (int64_t)row[u] * p.ncol + col[u] * 32 + 8 * a) = mx_values(codes, e);
         // ggml's block: e, then byte j = value j | value j + 16 << 4; lane a gets bytes 4a .. 4a + 3
@@ -190,7 +242,7 @@ __global__ __launch_bounds__(256) void k_mx_blocks(MxQuantArgs p) {
 
 // rows and tiles: a workgroup writes 512 columns of 16 rows, four pieces of 128; grid (np / 512, strips of the launch).
 // (Rows made block by block, a row's scales of 512 columns apart from the next row's in time and place, took 46 us of
-// 8192 x 7168 BF16 values, and MX_ROWS_US so: 16 rows' scales are two whole lines.)
+// 8192 x 7168 BF16 values, and 43 so: 16 rows' scales are two whole lines.)
 template <int SRC, bool TILES>
 __global__ __launch_bounds__(256) void k_mx_strips(MxQuantArgs p) {
     __shared__ uint32_t es[64];
@@ -198,12 +250,11 @@ __global__ __launch_bounds__(256) void k_mx_strips(MxQuantArgs p) {
     const uint32_t strip = (uint32_t)p.row0 + blockIdx.y, mat = p.row.div(strip);
     const int64_t in_mat = (int64_t)(strip - mat * p.row.d) * 16 + r, row = mat * p.nrow + in_mat;
     const bool has = in_mat < p.nrow;
-    float v[4][8];
-    uint32_t raw[4][3];
+    MxQuarter<SRC> v[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const uint32_t col = blockIdx.x * 16 + 4 * c + q;
-        mx_source<SRC>(p, row, col, has && col < p.nb, a, v[c], raw[c]);
+        v[c] = mx_source<SRC>(p, row, col, has && col < p.nb, a);
     }
     uint8_t *d = TILES ? p.dst + ((int64_t)strip * gridDim.x + blockIdx.x) * 4096 + (16 * q + r) * 16 + 4 * a
                        : p.dst + (row * gridDim.x + blockIdx.x) * 256 + 16 * q + 4 * a;
@@ -212,7 +263,7 @@ __global__ __launch_bounds__(256) void k_mx_strips(MxQuantArgs p) {
     for (int c = 0; c < 4; ++c) {
         const uint32_t col = blockIdx.x * 16 + 4 * c + q;
         uint32_t e;
-        const uint32_t codes = mx_encode<SRC>(a, v[c], raw[c], e);
+        const uint32_t codes = mx_encode<SRC>(a, v[c], e);
         all |= e << (8 * c);
         if (TILES || has) *(uint32_t *)(d + c * (TILES ? 1024 : 64)) = codes;
         if (p.values && has && col < p.nb)
@@ -236,13 +287,8 @@ __global__ __launch_bounds__(256) void k_mx_split(const void *__restrict__ src, 
     const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (c >= kp) return;
     for (int64_t r = blockIdx.y; r < nrow; r += gridDim.y) {
-        float v[8];
-        if (c < ncol) {
-            mx_load8<SRC>(src, r * ld + c, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        }
+        float v[8] = {};
+        if (c < ncol) mx_float8<SRC>(mx_load8<SRC>(src, r * ld + c), v);
 #pragma unroll
         for (int q = 0; q < PIECES; ++q) {
             uint32_t w[8];
