@@ -33,13 +33,17 @@ struct MxMulArgs {
 
 static __device__ __align__(16) uint32_t mx_zero[4];
 
-DEV uint32_t mx_bf16(float f) {          // to nearest even; NaN stays one
-    const uint32_t u = fbits(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
-    return (u + 0x7fffu + ((u >> 16) & 1)) >> 16;
-}
-DEV uint32_t mx_f16(float f) {
-    union { _Float16 h; uint16_t u; } c = {(_Float16)f};
+// four values as F16 or BF16, to nearest even
+DEV uint2 mx_halves(int type, const float (&v)[4]) {
+    if (type == T_BF16) {
+        union { __bf16 h[4]; uint2 u; } c;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c.h[k] = (__bf16)v[k];
+        return c.u;
+    }
+    union { _Float16 h[4]; uint2 u; } c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c.h[k] = (_Float16)v[k];
     return c.u;
 }
 
@@ -60,15 +64,13 @@ DEV void mx_store4(const MxMulArgs &a, int64_t row, int64_t n, const float (&v)[
         }
     } else {
         uint16_t *y = (uint16_t *)a.y + at;
-        uint32_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = a.ytype == T_BF16 ? mx_bf16(v[i]) : mx_f16(v[i]);
+        const uint2 h = mx_halves(a.ytype, v);
         if (whole) {
-            *(uint2 *)y = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+            *(uint2 *)y = h;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (n + i < a.ne1) y[i] = (uint16_t)h[i];
+                if (n + i < a.ne1) y[i] = (uint16_t)((i < 2 ? h.x : h.y) >> (16 * (i & 1)));
         }
     }
 }
@@ -395,38 +397,21 @@ DEV void mx_sync() {
 }
 
 // The tile's sums leave through LDS, GC fragments of every wave at a time, so that a store writes whole lines of a row
-// (16 bytes a lane of which four lanes share a row were 14 us of the 73 that 8192 x 2048 x 7168 takes with MXFP4 rows).
-// Rows that are not whole 16-byte pieces are stored value by value. lds: the loop's buffers, free by now.
-template <int WM, int WN, int FM, int FN, bool GLU>
-DEV void mx_epilogue(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0, int64_t r1, int64_t s0, uint8_t *lds) {
+// (straight from the registers four lanes share 64 bytes of a row). Rows that are not whole 16-byte pieces are stored value
+// by value. lds: the loop's buffers, free by now.
+template <int SIZE, int WM, int WN, int FM, int FN, bool GLU>
+DEV void mx_store_tile(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0, int64_t r1, int64_t s0, uint8_t *lds) {
     constexpr int FH = GLU ? FN / 2 : FN, NO = WN * FH * 16, GC = FM / 4, CR = WM * GC * 16;
+    constexpr int RB = NO * SIZE + 16, PER = 16 / SIZE, PIECES = NO / PER;      // a row in LDS; values and pieces of a row
     const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
-    if (a.part) {
-#pragma unroll
-        for (int g = 0; g < FM; ++g) {
-            const int64_t r = r0 + (wm * FM + g) * 16 + (lane & 15);
-            if (r >= r1) continue;
-            const bool on = mx_row(a, r) >= 0;
-#pragma unroll
-            for (int f = 0; f < FN; ++f) {
-                const int64_t n = (s0 + wn * FH + f % FH) * 16 + 4 * q;
-                float v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = on ? acc[f][g][k] : 0.f;
-                if (n < a.ne1) mx_part4(a, f / FH, r, n, v);
-            }
-        }
-        return;
-    }
-    const int size = a.ytype == T_F32 ? 4 : 2, rb = NO * size + 16, per = 16 / size;
-    const bool whole = a.ne1 % per == 0;
+    const bool whole = a.ne1 % PER == 0;
 #pragma unroll
     for (int g0 = 0; g0 < FM; g0 += GC) {
 #pragma unroll
         for (int i = 0; i < GC; ++i) {
             const int64_t r = r0 + (wm * FM + g0 + i) * 16 + (lane & 15);
             const bool on = r < r1 && mx_row(a, r) >= 0;
-            uint8_t *l = lds + ((wm * GC + i) * 16 + (lane & 15)) * rb + (wn * FH * 16 + 4 * q) * size;
+            uint8_t *l = lds + ((wm * GC + i) * 16 + (lane & 15)) * RB + (wn * FH * 16 + 4 * q) * SIZE;
 #pragma unroll
             for (int f = 0; f < FH; ++f) {
                 float v[4];
@@ -439,26 +424,49 @@ DEV void mx_epilogue(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0,
                 if (!whole) {
                     const int64_t n = (s0 + wn * FH + f) * 16 + 4 * q;
                     if (r < r1 && n < a.ne1) mx_store4(a, r, n, v);
-                } else if (size == 4) {
+                } else if (SIZE == 4) {
                     *(float4 *)(l + f * 64) = make_float4(v[0], v[1], v[2], v[3]);
                 } else {
-                    uint32_t h[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) h[k] = a.ytype == T_BF16 ? mx_bf16(v[k]) : mx_f16(v[k]);
-                    *(uint2 *)(l + f * 32) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+                    *(uint2 *)(l + f * 32) = mx_halves(a.ytype, v);
                 }
             }
         }
         if (!whole) continue;                               // (uniform)
         __syncthreads();
-        const int pieces = NO / per;                        // of a row
-        for (int i = tid; i < CR * pieces; i += WM * WN * 64) {
-            const int lr = i / pieces, p = i % pieces, w = lr / (GC * 16);
-            const int64_t r = r0 + (w * FM + g0) * 16 + lr % (GC * 16), n = s0 * 16 + p * per;
+#pragma unroll 4
+        for (int i = tid; i < CR * PIECES; i += WM * WN * 64) {
+            const int lr = i / PIECES, p = i % PIECES, w = lr / (GC * 16);
+            const int64_t r = r0 + (w * FM + g0) * 16 + lr % (GC * 16), n = s0 * 16 + p * PER;
             if (r < r1 && n < a.ne1)
-                *(uint4 *)((uint8_t *)a.y + (r * a.ne1 + n) * size) = *(const uint4 *)(lds + lr * rb + p * 16);
+                *(uint4 *)((uint8_t *)a.y + (r * a.ne1 + n) * SIZE) = *(const uint4 *)(lds + lr * RB + p * 16);
         }
         __syncthreads();
+    }
+}
+
+template <int WM, int WN, int FM, int FN, bool GLU>
+DEV void mx_epilogue(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0, int64_t r1, int64_t s0, uint8_t *lds) {
+    constexpr int FH = GLU ? FN / 2 : FN;
+    if (a.part) {
+        const int lane = lane_id(), wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+#pragma unroll
+        for (int g = 0; g < FM; ++g) {
+            const int64_t r = r0 + (wm * FM + g) * 16 + (lane & 15);
+            if (r >= r1) continue;
+            const bool on = mx_row(a, r) >= 0;
+#pragma unroll
+            for (int f = 0; f < FN; ++f) {
+                const int64_t n = (s0 + wn * FH + f % FH) * 16 + 4 * (lane >> 4);
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = on ? acc[f][g][k] : 0.f;
+                if (n < a.ne1) mx_part4(a, f / FH, r, n, v);
+            }
+        }
+    } else if (a.ytype == T_F32) {
+        mx_store_tile<4, WM, WN, FM, FN, GLU>(a, acc, r0, r1, s0, lds);
+    } else {
+        mx_store_tile<2, WM, WN, FM, FN, GLU>(a, acc, r0, r1, s0, lds);
     }
 }
 
