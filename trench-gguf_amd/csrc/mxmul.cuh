@@ -710,32 +710,37 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
             for (int f = 0; f < FN; ++f) wc[f] >>= 16;
         }
+        // two fragments of x at a time, the next two and the second half's weights on their way
+        constexpr int HP = FM / 2;
+        uint4 wv[2][FN], xv[2][2];
+        auto read = [&](int t) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint4 wv[FN], xv[2][2];
-            auto read = [&](int p) {
+            for (int i = 0; i < 2; ++i)
+                xv[t & 1][i] = *(const uint4 *)(x + (t % HP * 2 + i) * 2048 + ((4 * (t / HP) + q) ^ sw) * 16);
+        };
+        auto weights = [&](int h) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) xv[p & 1][i] = *(const uint4 *)(x + (2 * p + i) * 2048 + ((4 * h + q) ^ sw) * 16);
-            };
+            for (int f = 0; f < FN; ++f) wv[h][f] = *(const uint4 *)(w + f * 2048 + h * 1024);
+        };
+        weights(0);
+        read(0);
 #pragma unroll
-            for (int f = 0; f < FN; ++f) wv[f] = *(const uint4 *)(w + f * 2048 + h * 1024);
-            read(0);
+        for (int t = 0; t < 2 * HP; ++t) {
+            const int h = t / HP;
+            if (t + 1 < 2 * HP) read(t + 1);
+            if (t == HP - 2) weights(1);
 #pragma unroll
-            for (int p = 0; p < FM / 2; ++p) {
-                    if (p + 1 < FM / 2) read(p + 1);
+            for (int i = 0; i < 2; ++i) {
+                const int g = t % HP * 2 + i;
+                const mx_i8 xi = mx_wide(xv[t & 1][i]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int g = 2 * p + i;
-                    const mx_i8 xi = mx_wide(xv[p & 1][i]);
-#pragma unroll
-                    for (int f = 0; f < FN; ++f)
-                        acc[f][g] = h == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                                 mx_wide(wv[f]), xi, acc[f][g], 4, 4, 0, (int)wc[f], 0, (int)xc[g])
-                                           : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                                 mx_wide(wv[f]), xi, acc[f][g], 4, 4, 1, (int)wc[f], 1, (int)xc[g]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                for (int f = 0; f < FN; ++f)
+                    acc[f][g] = h == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                             mx_wide(wv[0][f]), xi, acc[f][g], 4, 4, 0, (int)wc[f], 0, (int)xc[g])
+                                       : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                             mx_wide(wv[1][f]), xi, acc[f][g], 4, 4, 1, (int)wc[f], 1, (int)xc[g]);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         mx_sync();
     }
