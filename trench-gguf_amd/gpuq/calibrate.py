@@ -1,0 +1,124 @@
+"""The Hessians of a mixture-of-experts layer, from calibration rows run through its stored MXFP4 experts on the device.
+
+    python calibrate.py <model.gguf> <layer> <rows dir> <out dir> --topk=K [--score=softmax|sigmoid] [--bias=<.npy>]
+                        [--groups=G --keep=N] [--chunk=4096] [--gpu=N]
+
+Error-feedback rounding of an expert needs the sum of x x^T over the rows the router sends it (gate and up), and over the
+hidden rows silu(gate x) * (up x) those become (down). The reference gets both from a dump of llama.cpp's own pass
+(tools/hessian_from_dump.py:58-151); here the layer's router logits and input rows are enough: the choice of experts, the
+grouping of the rows, both products with SwiGLU and the sums all run on the device (gpuq.experts,
+gpuq_hessian_accumulate_dev). <rows dir> holds blk.L.x.npy [n, ne0] (the rows that reach the experts, F32 or F16) and
+blk.L.logits.npy [n, nexp] (the router's, F32 or F16); <out dir> gets blk.L.in.npy [nexp, ne0, ne0], blk.L.mid.npy [nexp,
+nff, nff] and blk.L.counts.npy [nexp], the folder that requant.py's --hessian reads. The gate and up experts must be
+stored as MXFP4; ne0 and nff are whole 256s.
+"""
+import os
+import sys
+
+import numpy as np
+
+if __package__ in (None, ""):
+    sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+import gpuq  # noqa: E402
+
+
+class ExpertHessians:
+    """The Hessian sums of one layer's experts on the device.
+
+    gate, up: ggml's MXFP4 blocks of [nexp, nff, ne0] (uint8 on the device); topk and `choice` (score, bias, ngroup,
+    keep) as gpuq.experts.route takes them. `add` any number of chunks of rows, then read hin [nexp, ne0, ne0], hmid
+    [nexp, nff, nff] (f64, on the device) and counts [nexp], or `save` them."""
+
+    def __init__(self, gq, gate, up, nexp, nff, ne0, topk, **choice):
+        import torch
+        from gpuq import experts
+        if ne0 % 256 or nff % 256:
+            raise ValueError("Hessians take rows of whole 256s, not %d and %d" % (ne0, nff))
+        self.gq, self.nexp, self.nff, self.ne0, self.topk, self.choice = gq, nexp, nff, ne0, topk, choice
+        self.gate = experts.pack(gq, gate, nexp, nff, ne0)
+        self.up = experts.pack(gq, up, nexp, nff, ne0)
+        self.hin = torch.zeros((nexp, ne0, ne0), dtype=torch.float64, device=gate.device)
+        self.hmid = torch.zeros((nexp, nff, nff), dtype=torch.float64, device=gate.device)
+        self.counts = np.zeros(nexp, dtype=np.int64)
+
+    def _sum(self, rows, H):
+        import torch
+        rc = self.gq.gpuq_hessian_accumulate_dev(rows.data_ptr(), rows.shape[0], rows.shape[1], H.data_ptr(),
+                                                 torch.cuda.current_stream().cuda_stream)
+        if rc != 0:
+            raise RuntimeError("gpuq_hessian_accumulate_dev failed (%d)" % rc)
+
+    def add(self, x, logits):
+        """x [n, ne0] and logits [n, nexp] on the device (F32, F16 or BF16)"""
+        from gpuq import experts
+        ids, _ = experts.route(self.gq, logits, self.topk, **self.choice)
+        g = experts.group(self.gq, ids, self.nexp)
+        mid = experts.matmul(self.gq, x, self.gate, group=g, up=self.up)
+        offsets = g.offsets.tolist()
+        for e in range(self.nexp):
+            a, b = offsets[e], offsets[e + 1]
+            if a == b:
+                continue
+            self._sum(x.index_select(0, g.rows[a:b].long()).float(), self.hin[e])
+            self._sum(mid[a:b], self.hmid[e])
+            self.counts[e] += b - a
+
+    def save(self, out_dir, layer):
+        os.makedirs(out_dir, exist_ok=True)
+        for name, H in (("in", self.hin), ("mid", self.hmid)):
+            out = np.lib.format.open_memmap(os.path.join(out_dir, "blk.%d.%s.npy" % (layer, name)), mode="w+",
+                                            dtype=np.float64, shape=tuple(H.shape))
+            for e in range(self.nexp):              # (an expert at a time: a layer's sums can be 100 GB)
+                out[e] = H[e].cpu().numpy()
+            out.flush()
+        np.save(os.path.join(out_dir, "blk.%d.counts.npy" % layer), self.counts.astype(np.float64))
+
+
+def run(model, layer, rows_dir, out_dir, topk, gq=None, device=0, chunk=4096, **choice):
+    """one layer of a GGUF file; returns its ExpertHessians"""
+    import torch
+    from gpuq import gguf_io
+    gq = gq or gpuq.load_gpuq(device)
+    reader = gguf_io.GGUFReader(model)
+    blocks, shapes = [], []
+    for part in ("gate", "up"):
+        t = reader.tensor("blk.%d.ffn_%s_exps.weight" % (layer, part))
+        if t.tensor_type != gpuq.MXFP4:
+            raise ValueError("%s is stored as %s, not MXFP4" % (t.name, gguf_io.type_name(t.tensor_type)))
+        blocks.append(torch.from_numpy(np.array(t.data)).cuda(device))
+        shapes.append(t.shape)
+    if shapes[0] != shapes[1]:
+        raise ValueError("gate and up experts differ: %s, %s" % tuple(shapes))
+    ne0, nff, nexp = shapes[0]
+    x = np.load(os.path.join(rows_dir, "blk.%d.x.npy" % layer), mmap_mode="r")
+    logits = np.load(os.path.join(rows_dir, "blk.%d.logits.npy" % layer), mmap_mode="r")
+    if x.shape[1:] != (ne0,) or logits.shape != (len(x), nexp):
+        raise ValueError("rows %s and logits %s do not fit %d experts of %d columns" % (x.shape, logits.shape, nexp, ne0))
+    if choice.get("bias") is not None:
+        choice["bias"] = torch.from_numpy(np.ascontiguousarray(choice["bias"], dtype=np.float32)).cuda(device)
+    h = ExpertHessians(gq, blocks[0], blocks[1], nexp, nff, ne0, topk, **choice)
+    for i in range(0, len(x), chunk):
+        h.add(torch.from_numpy(np.array(x[i:i + chunk])).cuda(device), torch.from_numpy(np.array(logits[i:i + chunk])).cuda(device))
+    h.save(out_dir, layer)
+    return h
+
+
+def main(argv):
+    opt = dict(a.split("=", 1) for a in argv if a.startswith("--") and "=" in a)
+    args = [a for a in argv if not a.startswith("--")]
+    known = ("--topk", "--score", "--bias", "--groups", "--keep", "--chunk", "--gpu")
+    if len(args) != 4 or "--topk" not in opt or any(k not in known for k in opt) or \
+            len(args) + len(opt) != len(argv):
+        print(__doc__.split("\n\n")[1], file=sys.stderr)
+        return 2
+    choice = {"score": opt.get("--score", "softmax"), "ngroup": int(opt.get("--groups", 1)), "keep": int(opt.get("--keep", 1))}
+    if "--bias" in opt:
+        choice["bias"] = np.load(opt["--bias"])
+    h = run(args[0], int(args[1]), args[2], args[3], int(opt["--topk"]), device=int(opt.get("--gpu", 0)),
+            chunk=int(opt.get("--chunk", 4096)), **choice)
+    print("layer %s: %d rows to %d of %d experts" % (args[1], int(h.counts.sum()), int((h.counts > 0).sum()), h.nexp))
+    return 0
+
+
+if __name__ == "__main__":
+    sys.exit(main(sys.argv[1:]))
