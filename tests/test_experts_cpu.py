@@ -14,9 +14,10 @@ def test_sizes(lib):
     assert lib.gpuq_mxfp4_bytes(2, 256, 2048, 7168) == 256 * 2048 * 7168 * 17 // 32
     assert [lib.gpuq_mxfp4_bytes(*a) for a in ((0, 1, 0, 32), (1, 0, 1, 32), (2, 1, 1, 33), (1, 1, -1, 32), (3, 1, 1, 32),
                                                (-1, 1, 1, 32), (0, 1, 1, 1 << 25), (2, 1 << 20, 1 << 20, 32))] == [0] * 8
-    # F32 and F16 rows as 3 and 2 BF16 rows of whole 128s; partial sums only where there are few tiles
-    assert [lib.gpuq_mxfp4_matmul_work(t, 0, 10, 1, 64, 3200, 0, 10) for t in (0, 1, 30, 39)] == [192000, 128000, 0, 0]
-    assert lib.gpuq_mxfp4_matmul_work(0, 0, 3, 1, 64, 32, 0, 3) == 3 * 128 * 6
+    # many F32 and F16 rows as 3 and 2 BF16 rows of whole 128s; partial sums only where there are few tiles
+    assert [lib.gpuq_mxfp4_matmul_work(t, 0, 8192, 1, 8192, 3200, 0, 8192) for t in (0, 1, 30, 39)] == [8192 * 19200,
+                                                                                                   8192 * 12800, 0, 0]
+    assert [lib.gpuq_mxfp4_matmul_work(t, 0, 16, 1, 64, 32, 0, 16) for t in (0, 1, 30, 39)] == [0] * 4
     part = lib.gpuq_mxfp4_matmul_work(30, 0, 100, 1, 64, 4096, 0, 100)
     assert part > 0 and part % (100 * 64 * 4) == 0 and lib.gpuq_mxfp4_matmul_work(30, 1, 100, 1, 64, 4096, 0, 100) % part == 0
     assert lib.gpuq_mxfp4_matmul_work(30, 0, 8192, 1, 8192, 4096, 0, 8192) == 0

@@ -621,7 +621,7 @@ def test_refusals(gq, ex):
         args = list(good)
         args[at] = bad
         assert mm(*args) == 0, (at, bad)
-    assert mm(F32, p, 16, 512, o, None, 1, 32, 512, None, None, 16, F32, o, None, st) == 0      # no scratch
+    assert mm(F32, p, 32, 512, o, None, 1, 32, 512, None, None, 32, F32, o, None, st) == 0      # no scratch
     r = gq.gpuq_route_dev
     assert r(F32, p, 4, 64, 64, 2, 0, None, 1, 1, 1, 1.0, o, o + 1024, st) == 0
     good = [F32, p, 4, 64, 64, 2, 0, None, 1, 1, 1, 1.0, o, o + 1024, st]

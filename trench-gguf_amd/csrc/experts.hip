@@ -43,17 +43,18 @@ bool sizes_ok(int64_t nx, int64_t nmat, int64_t ne1, int64_t ne0, int64_t m) {
            nx > 0 && nx <= MAX_ROWS && m > 0 && m <= MAX_ROWS;
 }
 
-template <int MF, int NF> void launch_rows(bool fp4, bool glu, const MxMulArgs &a, hipStream_t st) {
+template <int SRC, int NF> void launch_rows_of(bool glu, const MxMulArgs &a, hipStream_t st) {
     const dim3 grid((unsigned)((a.strips + NF - 1) / NF), (unsigned)(a.offsets ? std::min(a.nmat, a.m) + 1 : 1));
-#define MX_ROWS_K(F, G) hipLaunchKernelGGL((k_mx_rows<F, MF, NF, G>), grid, dim3(512), 0, st, a)
-    if (fp4) {
-        if (glu) MX_ROWS_K(true, true);
-        else MX_ROWS_K(true, false);
-    } else {
-        if (glu) MX_ROWS_K(false, true);
-        else MX_ROWS_K(false, false);
+    if (glu) hipLaunchKernelGGL((k_mx_rows<SRC, NF, true>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_mx_rows<SRC, NF, false>), grid, dim3(512), 0, st, a);
+}
+template <int NF> void launch_rows(int x_type, bool glu, const MxMulArgs &a, hipStream_t st) {
+    switch (x_type) {
+        case T_F32: launch_rows_of<T_F32, NF>(glu, a, st); break;
+        case T_F16: launch_rows_of<T_F16, NF>(glu, a, st); break;
+        case T_BF16: launch_rows_of<T_BF16, NF>(glu, a, st); break;
+        default: launch_rows_of<T_MXFP4, NF>(glu, a, st);
     }
-#undef MX_ROWS_K
 }
 
 // How a product runs. A workgroup of k_mx_rows reads its strips' weights once for every 16 rows of a group: right for
@@ -176,7 +177,7 @@ extern "C" size_t gpuq_mxfp4_matmul_work(int x_type, int glu, int64_t nx, int64_
     if ((x_type != T_MXFP4 && !float_type(x_type)) || !sizes_ok(nx, nmat, ne1, ne0, m) ||
         !plan_product(x_type, glu != 0, nmat, ne1, ne0, m, grouped != 0, p))
         return 0;
-    return pieces_bytes(x_type, nx, ne0) + p.part;
+    return (p.kind ? pieces_bytes(x_type, nx, ne0) : 0) + p.part;
 }
 
 extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx, int64_t ld, const void *d_w,
@@ -190,11 +191,10 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
         ((uintptr_t)d_rows & 3))
         return 0;
     if (fp4 ? ld != ne0 : ld < ne0 || ld > ((int64_t)1 << 40) || ld * type_size(x_type) % 16) return 0;
-    const int pieces = pieces_of(x_type);
     const bool glu = d_up != nullptr;
     Plan plan;
     if (!plan_product(x_type, glu, nmat, ne1, ne0, m, d_offsets != nullptr, plan)) return 0;
-    const size_t px = pieces_bytes(x_type, nx, ne0);
+    const size_t px = plan.kind ? pieces_bytes(x_type, nx, ne0) : 0;
     if ((px + plan.part) && (!d_work || !aligned16(d_work))) return 0;
     const hipStream_t st = (hipStream_t)stream;
     const int64_t np = mx_padded(ne0), strips = strips_of(ne1), wcodes = nmat * strips * 8 * np;
@@ -214,30 +214,29 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
     a.m = m;
     a.y = d_y;
     a.ytype = y_type;
-    a.pieces = pieces;
+    a.pieces = 1;
+    a.x = (const uint8_t *)d_x;
     if (fp4) {
-        a.x = (const uint8_t *)d_x;
         a.xs = a.x + nx * (np / 2);
         a.xrow = np / 2;
-    } else if (pieces == 1) {
-        a.x = (const uint8_t *)d_x;
-        a.xrow = ld * 2;
-        a.kx = ne0;
     } else {
+        a.xrow = ld * type_size(x_type);
+        a.kx = ne0;
+    }
+    if (px) {
         const int64_t kp = round128(ne0);
         const dim3 grid((unsigned)((kp / 8 + 255) / 256), (unsigned)(nx < 65535 ? nx : 65535));
-        if (x_type == T_F32)
-            hipLaunchKernelGGL((k_mx_split<T_F32, 3>), grid, dim3(256), 0, st, d_x, ld, ne0, kp, nx, (uint16_t *)d_work);
-        else
-            hipLaunchKernelGGL((k_mx_split<T_F16, 2>), grid, dim3(256), 0, st, d_x, ld, ne0, kp, nx, (uint16_t *)d_work);
+        if (x_type == T_F32) hipLaunchKernelGGL(k_mx_split<T_F32>, grid, dim3(256), 0, st, d_x, ld, ne0, kp, nx, (uint16_t *)d_work);
+        else hipLaunchKernelGGL(k_mx_split<T_F16>, grid, dim3(256), 0, st, d_x, ld, ne0, kp, nx, (uint16_t *)d_work);
+        a.pieces = pieces_of(x_type);
         a.x = (const uint8_t *)d_work;
-        a.xrow = kp * 2 * pieces;
-        a.kx = kp * pieces;
+        a.xrow = kp * 2 * a.pieces;
+        a.kx = kp * a.pieces;
     }
     if (plan.kind == 0) {
         // four strips a workgroup where that leaves two for every CU
-        if (a.strips * std::min(nmat, m) >= 2048) launch_rows<1, 4>(fp4, glu, a, st);
-        else launch_rows<1, 1>(fp4, glu, a, st);
+        if (a.strips * std::min(nmat, m) >= 2048) launch_rows<4>(x_type, glu, a, st);
+        else launch_rows<1>(x_type, glu, a, st);
     } else {
         a.mt = (int)plan.mt;
         a.part = plan.split > 1 ? (float *)((uint8_t *)d_work + px) : nullptr;

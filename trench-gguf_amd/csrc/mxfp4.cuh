@@ -278,29 +278,34 @@ __global__ __launch_bounds__(256) void k_mx_strips(MxQuantArgs p) {
     }
 }
 
-// F32 / F16 rows as sums of BF16 rows: the top 16 bits, then those of the rest, which holds every bit of an F16 value
-// in 2 pieces and of an F32 value in 3 (8 bits each). out [nrow][PIECES][kp], kp = ncol rounded up to 128, zero-padded;
-// one lane 8 values; grid (ceil(kp / 8 / 256), rows)
-template <int SRC, int PIECES>
+// F32 / F16 values as sums of BF16 values: the top 16 bits, then those of the rest, which holds every bit of an F16 value
+// in 2 pieces and of an F32 value in 3 (8 bits each)
+template <int SRC> struct MxPieces { static constexpr int n = SRC == T_F32 ? 3 : SRC == T_F16 ? 2 : 1; };
+// the next piece of 8 values, taken off them
+DEV uint4 mx_piece(float (&v)[8]) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = fbits(v[j]);
+        const bool fin = (b & 0x7f800000u) != 0x7f800000u;
+        w[j] = (b >> 16) | (!fin && (b & 0x7fffffu) ? 0x40u : 0u);      // (a NaN stays one)
+        v[j] = fin ? v[j] - ffrom(b & 0xffff0000u) : 0.f;
+    }
+    return make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+}
+
+// rows in pieces: out [nrow][pieces][kp], kp = ncol rounded up to 128, zero-padded; one lane 8 values; grid (ceil(kp / 8 /
+// 256), rows)
+template <int SRC>
 __global__ __launch_bounds__(256) void k_mx_split(const void *__restrict__ src, int64_t ld, int64_t ncol, int64_t kp,
                                                   int64_t nrow, uint16_t *__restrict__ out) {
+    constexpr int N = MxPieces<SRC>::n;
     const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (c >= kp) return;
     for (int64_t r = blockIdx.y; r < nrow; r += gridDim.y) {
         float v[8] = {};
         if (c < ncol) mx_float8<SRC>(mx_load8<SRC>(src, r * ld + c), v);
 #pragma unroll
-        for (int q = 0; q < PIECES; ++q) {
-            uint32_t w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t b = fbits(v[j]);
-                const bool fin = (b & 0x7f800000u) != 0x7f800000u;
-                w[j] = (b >> 16) | (!fin && (b & 0x7fffffu) ? 0x40u : 0u);      // (a NaN stays one)
-                v[j] = fin ? v[j] - ffrom(b & 0xffff0000u) : 0.f;
-            }
-            *(uint4 *)(out + (r * PIECES + q) * kp + c) =
-                make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
-        }
+        for (int q = 0; q < N; ++q) *(uint4 *)(out + (r * N + q) * kp + c) = mx_piece(v);
     }
 }

@@ -168,8 +168,10 @@ DEV uint32_t mx_opaque(uint32_t v) {
 }
 
 // ---- few rows a group: a workgroup owns NF strips of one group, its 8 waves split k by 128-value pieces and their sums
-// meet in LDS in a fixed order; MF x 16 rows at a time. The weights' bytes bound it, so each wave keeps the loads of two
-// pieces ahead of its products in flight. grid (ceil(strips / NF), groups that can have rows + 1)
+// meet in LDS in a fixed order; 16 rows at a time. F32 and F16 rows become pieces on the way to the products. The weights'
+// bytes bound it, so each wave keeps the loads of a piece ahead of its products in flight, and a workgroup takes four
+// strips where there are enough of them, since x costs as much to load as they (8 tokens over 256 experts of 2048 x 7168:
+// 120 us with one strip, 88 with four, 5.1 TB/s). grid (ceil(strips / NF), groups that can have rows + 1)
 
 // the y-th group that has rows (the last workgroup row: the rows of no group); false where there is none
 DEV bool mx_group_at(const MxMulArgs &a, int y, int64_t &e, int64_t &r0, int64_t &r1) {
@@ -203,10 +205,12 @@ DEV bool mx_group_at(const MxMulArgs &a, int y, int64_t &e, int64_t &r0, int64_t
     return false;
 }
 
-template <bool FP4, int MF, int NF, bool GLU>
+template <int SRC, int NF, bool GLU>
 __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
-    constexpr int G = NF * (GLU ? 2 : 1), D = 2;      // streams of weights; pieces in flight
-    __shared__ mx_f4 red[8][MF * G][64];
+    constexpr bool FP4 = SRC == T_MXFP4;
+    constexpr int G = NF * (GLU ? 2 : 1), D = 2, XR = FP4 ? 1 : 4;  // streams of weights, pieces in flight
+    constexpr int XS = SRC == T_F32 ? T_F32 : SRC == T_F16 ? T_F16 : T_BF16, SIZE = SRC == T_F32 ? 4 : 2;
+    __shared__ mx_f4 red[8][G][64];
     const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t s0 = (int64_t)blockIdx.x * NF;
@@ -223,99 +227,95 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
         wp[g] = (g < NF ? a.w : a.u) + strip * a.nc * 4096;
         sp[g] = (g < NF ? a.ws : a.us) + strip * a.nc * 256;
     }
-    const int total = FP4 ? a.nk : a.nk * a.pieces;
-    for (int64_t m0 = r0; m0 < r1; m0 += 16 * MF) {
-        mx_f4 acc[MF][G];
-        const uint8_t *xp[MF], *xsp[MF];
+    for (int64_t m0 = r0; m0 < r1; m0 += 16) {
+        mx_f4 acc[G];
+        const int64_t r = m0 + (lane & 15);
+        const int64_t i = mx_row(a, r < r1 ? r : r1 - 1);
+        const uint8_t *xp = a.x + (i < 0 ? 0 : i) * a.xrow + (FP4 ? 16 : 32 * SIZE) * q;
+        const uint8_t *xsp = FP4 ? a.xs + (i < 0 ? 0 : i) * 16 + 4 * q : nullptr;
 #pragma unroll
-        for (int f = 0; f < MF; ++f) {
-            const int64_t r = m0 + 16 * f + (lane & 15);
-            const int64_t i = mx_row(a, r < r1 ? r : r1 - 1);
-            xp[f] = a.x + (i < 0 ? 0 : i) * a.xrow + (FP4 ? 16 : 64) * q;
-            xsp[f] = FP4 ? a.xs + (i < 0 ? 0 : i) * 16 + 4 * q : nullptr;
-#pragma unroll
-            for (int g = 0; g < G; ++g) acc[f][g] = mx_f4{0.f, 0.f, 0.f, 0.f};
-        }
-        uint4 wq[D][G], xv[D][MF][FP4 ? 1 : 4];
-        uint32_t sc[D][G], xc[D][MF];
-        auto load = [&](int s, int d) {     // piece s
-            const int c = FP4 ? s : s % a.nk;
+        for (int g = 0; g < G; ++g) acc[g] = mx_f4{0.f, 0.f, 0.f, 0.f};
+        uint4 wq[D][G];
+        MxRaw<XS> xv[D][XR];
+        uint32_t sc[D][G], xc[D];
+        auto load = [&](int c, int d) {     // piece c
             const uint32_t at = mx_opaque(16u * (uint32_t)lane);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 wq[d][g] = *(const uint4 *)(wp[g] + (int64_t)c * 1024 + at);
                 sc[d][g] = *(sp[g] + (int64_t)(c >> 2) * 256 + ((c & 3) + (at >> 2)));
             }
+            if (FP4) {
+                xv[d][0] = mx_load8<XS>(xp + (int64_t)c * 64, 0);
+                xc[d] = xsp[(int64_t)(c >> 2) * a.nx * 16 + (c & 3)];
+            } else {
+                const bool in = (int64_t)c * 128 + 32 * q < a.kx;
+                const uint8_t *x = in ? xp + (int64_t)c * 128 * SIZE : (const uint8_t *)mx_zero;
 #pragma unroll
-            for (int f = 0; f < MF; ++f) {
-                if (FP4) {
-                    xv[d][f][0] = *(const uint4 *)(xp[f] + (int64_t)c * 64);
-                    xc[d][f] = xsp[f][(int64_t)(c >> 2) * a.nx * 16 + (c & 3)];
-                } else {
-                    const bool in = (int64_t)s * 128 + 32 * q < a.kx;
-#pragma unroll
-                    for (int j = 0; j < (FP4 ? 1 : 4); ++j)
-                        xv[d][f][j] = *(const uint4 *)(in ? xp[f] + (int64_t)s * 256 + 16 * j : (const uint8_t *)mx_zero);
-                }
+                for (int j = 0; j < XR; ++j) xv[d][j] = mx_load8<XS>(x, in ? 8 * j : 0);
             }
         };
         auto work = [&](int d) {
+            if constexpr (FP4) {
+                const uint4 xi = make_uint4(xv[d][0].w[0], xv[d][0].w[1], xv[d][0].w[2], xv[d][0].w[3]);
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                if (FP4) {
+                for (int g = 0; g < G; ++g)
+                    acc[g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_wide(wq[d][g]), mx_wide(xi), acc[g], 4, 4, 0,
+                                                                              (int)sc[d][g], 0, (int)xc[d]);
+            } else {
 #pragma unroll
-                    for (int f = 0; f < MF; ++f)
-                        acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                            mx_wide(wq[d][g]), mx_wide(xv[d][f][0]), acc[f][g], 4, 4, 0, (int)sc[d][g], 0, (int)xc[d][f]);
-                } else {
-                    const float scale = ffrom(sc[d][g] << 23);
-                    const uint32_t cw[4] = {wq[d][g].x, wq[d][g].y, wq[d][g].z, wq[d][g].w};
+                for (int j = 0; j < XR; ++j) {
+                    constexpr int N = MxPieces<XS>::n;
+                    union { uint4 u; mx_bf8 b; } x[N];
+                    if constexpr (N == 1) {
+                        x[0].u = make_uint4(xv[d][j].w[0], xv[d][j].w[1], xv[d][j].w[2], xv[d][j].w[3]);
+                    } else {
+                        float v[8];
+                        mx_float8<XS>(xv[d][j], v);
 #pragma unroll
-                    for (int j = 0; j < (FP4 ? 1 : 4); ++j) {
-                        const mx_bf8 wv = mx_widen(cw[j], scale);
+                        for (int p = 0; p < N; ++p) x[p].u = mx_piece(v);
+                    }
 #pragma unroll
-                        for (int f = 0; f < MF; ++f) {
-                            union { uint4 u; mx_bf8 b; } x = {xv[d][f][j]};
-                            acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, x.b, acc[f][g], 0, 0, 0);
-                        }
+                    for (int g = 0; g < G; ++g) {
+                        const uint32_t cw = j == 0 ? wq[d][g].x : j == 1 ? wq[d][g].y : j == 2 ? wq[d][g].z : wq[d][g].w;
+                        const mx_bf8 wv = mx_widen(cw, ffrom(sc[d][g] << 23));
+#pragma unroll
+                        for (int p = 0; p < N; ++p)
+                            acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, x[p].b, acc[g], 0, 0, 0);
                     }
                 }
             }
         };
 #pragma unroll
         for (int d = 0; d < D - 1; ++d)
-            if (wave + 8 * d < total) load(wave + 8 * d, d);
-        for (int s = wave; s < total; s += 8 * D) {
+            if (wave + 8 * d < a.nk) load(wave + 8 * d, d);
+        for (int c = wave; c < a.nk; c += 8 * D) {
 #pragma unroll
             for (int d = 0; d < D; ++d) {
-                const int ahead = s + 8 * (d + D - 1);
-                if (ahead < total) load(ahead, (d + D - 1) % D);
-                if (s + 8 * d < total) work(d);
+                const int ahead = c + 8 * (d + D - 1);
+                if (ahead < a.nk) load(ahead, (d + D - 1) % D);
+                if (c + 8 * d < a.nk) work(d);
             }
         }
 #pragma unroll
-        for (int f = 0; f < MF; ++f)
-#pragma unroll
-            for (int g = 0; g < G; ++g) red[wave][f * G + g][lane] = acc[f][g];
+        for (int g = 0; g < G; ++g) red[wave][g][lane] = acc[g];
         __syncthreads();
-        for (int i = wave; i < MF * NF; i += 8) {           // fragment f of strip k
-            const int f = i / NF, k = i % NF;
+        if (wave < NF) {                                    // a wave a strip
             float v[2][4];
 #pragma unroll
             for (int h = 0; h < (GLU ? 2 : 1); ++h) {
-                mx_f4 sum = red[0][f * G + h * NF + k][lane];
+                mx_f4 sum = red[0][h * NF + wave][lane];
 #pragma unroll
-                for (int w = 1; w < 8; ++w) sum += red[w][f * G + h * NF + k][lane];
+                for (int w = 1; w < 8; ++w) sum += red[w][h * NF + wave][lane];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[h][j] = sum[j];
             }
-            const int64_t r = m0 + 16 * f + (lane & 15), n = (s0 + k) * 16 + 4 * q;
+            const int64_t n = (s0 + wave) * 16 + 4 * q;
             if (r < r1 && n < a.ne1) {
-                const bool on = mx_row(a, r) >= 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (GLU) v[0][j] = mx_glu(v[0][j], v[GLU ? 1 : 0][j]);
-                    if (!on) v[0][j] = 0.f;
+                    if (i < 0) v[0][j] = 0.f;
                 }
                 mx_store4(a, r, n, v[0]);
             }
