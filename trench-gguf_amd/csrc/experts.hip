@@ -57,9 +57,14 @@ template <int NF> void launch_rows(int x_type, bool glu, const MxMulArgs &a, hip
     }
 }
 
-// How a product runs. A workgroup of k_mx_rows reads its strips' weights once for every 16 rows of a group: right for
-// groups of a few rows. The tile kernels read them once for 64 to 256, and where their tiles are fewer than the GPU takes
-// at once, split k and join the partial sums.
+// How a product runs. k_mx_rows reads a group's weights once for every 16 of its rows: right for groups of a few rows. The
+// tile kernels read them once for 64 to 256, and where their tiles are fewer than the GPU takes at once, they split k and
+// join the partial sums. Both sides of each bound (us; experts of 2048 x 7168, 64 of them, 8 a token):
+//   8 rows a group on average, at most: k_mx_rows 112, tiles of 64 rows 120; at 16 166 and 124, at 1 67 and 104.
+//   One matrix: 16 rows 10.8 in k_mx_rows, 17 rows 16.8 in split tiles (unsplit 73).
+//   Tiles of 128 rows from 1024 of them on, two rounds of two a CU: 4096 rows of 2048 x 7168 (256 tiles) 116, with 64 rows
+//   98; 64 experts of 512 rows, SwiGLU (4600) 1.61 ms, with 64 rows 1.64.
+//   MXFP4 rows: 256 x 256 tiles where each group has 256 rows and they fill the GPU (8192 rows 72, with 128 x 128 78).
 struct Plan {
     int kind;                   // 0 k_mx_rows; tiles of 64 (1) or 128 (2) BF16 rows, 128 (3) or 256 (4) MXFP4 rows
     int tm, tn;
@@ -234,8 +239,13 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
         a.kx = kp * a.pieces;
     }
     if (plan.kind == 0) {
-        // four strips a workgroup where that leaves two for every CU
-        if (a.strips * std::min(nmat, m) >= 2048) launch_rows<4>(x_type, glu, a, st);
+        // strips a workgroup: x is loaded (and F32 rows made pieces) once for all of them, but the fewer workgroups the
+        // longer each reads. Kernel times of 13 rows of 7168 x 2048, 448 strips: F32 11.1, 8.1, 9.0 us with 1, 2 and 4,
+        // BF16 6.5, 5.3, 6.0; a row of 2048 x 7168, 128 strips: BF16 5.6, 6.6, 9.3; 8 tokens over 256 experts, some 7300:
+        // BF16 161, 110, 90
+        const int64_t n = a.strips * std::min(nmat, m);
+        if (n >= 2048) launch_rows<4>(x_type, glu, a, st);
+        else if (n >= 256) launch_rows<2>(x_type, glu, a, st);
         else launch_rows<1>(x_type, glu, a, st);
     } else {
         a.mt = (int)plan.mt;

@@ -281,17 +281,19 @@ __global__ __launch_bounds__(256) void k_mx_strips(MxQuantArgs p) {
 // F32 / F16 values as sums of BF16 values: the top 16 bits, then those of the rest, which holds every bit of an F16 value
 // in 2 pieces and of an F32 value in 3 (8 bits each)
 template <int SRC> struct MxPieces { static constexpr int n = SRC == T_F32 ? 3 : SRC == T_F16 ? 2 : 1; };
-// the next piece of 8 values, taken off them
-DEV uint4 mx_piece(float (&v)[8]) {
+// the next piece of 8 values, taken off them: the FIRST of an infinity is all of it and that of a NaN a NaN
+template <bool FIRST> DEV uint4 mx_piece(float (&v)[8]) {
     uint32_t w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const uint32_t b = fbits(v[j]);
-        const bool fin = (b & 0x7f800000u) != 0x7f800000u;
-        w[j] = (b >> 16) | (!fin && (b & 0x7fffffu) ? 0x40u : 0u);      // (a NaN stays one)
-        v[j] = fin ? v[j] - ffrom(b & 0xffff0000u) : 0.f;
+        const float hi = ffrom(fbits(v[j]) & 0xffff0000u);
+        const bool fin = !FIRST || fabsf(v[j]) < __builtin_inff();
+        w[j] = fin ? fbits(v[j]) : fbits(v[j] + v[j]);      // (a NaN gets the bit that the cut leaves)
+        v[j] = fin ? v[j] - hi : 0.f;
     }
-    return make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+#define MX_PAIR(I) __builtin_amdgcn_perm(w[I + 1], w[I], 0x07060302u)
+    return make_uint4(MX_PAIR(0), MX_PAIR(2), MX_PAIR(4), MX_PAIR(6));
+#undef MX_PAIR
 }
 
 // rows in pieces: out [nrow][pieces][kp], kp = ncol rounded up to 128, zero-padded; one lane 8 values; grid (ceil(kp / 8 /
@@ -305,7 +307,8 @@ __global__ __launch_bounds__(256) void k_mx_split(const void *__restrict__ src, 
     for (int64_t r = blockIdx.y; r < nrow; r += gridDim.y) {
         float v[8] = {};
         if (c < ncol) mx_float8<SRC>(mx_load8<SRC>(src, r * ld + c), v);
+        *(uint4 *)(out + r * N * kp + c) = mx_piece<true>(v);
 #pragma unroll
-        for (int q = 0; q < N; ++q) *(uint4 *)(out + (r * N + q) * kp + c) = mx_piece(v);
+        for (int q = 1; q < N; ++q) *(uint4 *)(out + (r * N + q) * kp + c) = mx_piece<false>(v);
     }
 }

@@ -1,10 +1,10 @@
 // trench-gguf_amd/csrc/mxmul.cuh - products of rows with stored MXFP4 matrices: y[r][n] = sum_k x[r][k] w[e][n][k],
 // with e the matrix of r's group, and with SwiGLU of two such products, y = g / (1 + exp(-g)) * u.
 //
-// The weights come packed (mxfp4.cuh). BF16 rows meet them as BF16: a code times its scale is exact there, products are
-// exact in f32 and the sums are held in f32. F32 and F16 rows come as sums of 3 and 2 BF16 rows (k_mx_split), summed
-// piece by piece into the same f32 sums, so no bit of them is lost. Packed MXFP4 rows meet the packed weights in the
-// scaled matrix instructions. A product is a matrix instruction with w's rows as its rows and x's as its columns, so a
+// The weights come in tiles (mxfp4.cuh). BF16 rows meet them as BF16: a code times its scale is exact there, products are
+// exact in f32 and the sums are held in f32. F32 and F16 values become sums of 3 and 2 BF16 values, all of them summed
+// into the same f32 sums, so no bit of them is lost. MXFP4 rows meet the weights' codes in the scaled matrix
+// instructions. A product is a matrix instruction with w's rows as its rows and x's as its columns, so a
 // lane ends up with 4 consecutive outputs of one row. The order of k inside an instruction is free as long as both
 // sides agree: lane group q takes k = 32 q .. 32 q + 31 of every 128, which are one 16-byte piece of codes under one
 // scale, and instruction c of four takes 8 c .. 8 c + 7 of those.
@@ -31,7 +31,7 @@ struct MxMulArgs {
     float *part;                // partial sums [split][1, with SwiGLU 2][m][ne1] of tiles whose k the grid's y splits, or null
 };
 
-static __device__ __align__(16) uint32_t mx_zero[4];
+static __device__ __align__(16) uint32_t mx_zero[8];      // what lies past the end of a row (8 values)
 
 // four values as F16 or BF16, to nearest even
 DEV uint2 mx_halves(int type, const float (&v)[4]) {
@@ -272,8 +272,9 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxMulArgs a) {
                     } else {
                         float v[8];
                         mx_float8<XS>(xv[d][j], v);
+                        x[0].u = mx_piece<true>(v);
 #pragma unroll
-                        for (int p = 0; p < N; ++p) x[p].u = mx_piece(v);
+                        for (int p = 1; p < N; ++p) x[p].u = mx_piece<false>(v);
                     }
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
@@ -474,7 +475,11 @@ DEV void mx_epilogue(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0,
 // second the same columns of u). x goes through LDS, 128 values of every row a step, in two buffers: piece 4q + c of a
 // row's 16, which lane group q takes into product c, lies at (4c + q) ^ (row & 15), so that the reads of 16 rows spread
 // over the banks. A wave's weights go straight to its registers, a kilobyte of a strip at a time and one ahead: as codes
-// they are a quarter of what the rows take, and no two waves read the same.
+// they are a quarter of what the rows take, and no two waves read the same. The matrix instructions and the power they
+// draw bound it: 64 experts of 512 rows with SwiGLU keep them busy for two thirds of the time at 1.9 GHz, 1.2 PFLOP/s of
+// the 1.4 that the library's product of BF16 rows and weights of that size reaches; 4096 x 2048 x 7168 takes 98 to 105 us,
+// the library's 107. Two workgroups a CU cover each other's waits; eight waves of one that take turns between LDS and
+// the products took 130 to 200 us there.
 template <int WN, int FM, int FN, bool GLU>
 DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int64_t s0, uint8_t *xs) {
     constexpr int TM = FM * 16, FH = GLU ? FN / 2 : FN, LD = TM / 4 / WN, HP = FM / 2;
@@ -606,7 +611,9 @@ __global__ __launch_bounds__(WN * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
 // MXFP4 rows: WM x WN waves, each FM x 16 rows by FN x 16 columns. Both sides are codes and as large, and the products
 // take a quarter of the BF16 ones' time, so both go through LDS (nothing is read twice), 256 values of k a step in two
 // buffers, and every load has a step's time. A row of x is 8 pieces of 16 bytes, piece p at p ^ (row / 2 & 7); a strip's
-// kilobytes lie as they are stored. The scales of 512 values follow every second step.
+// kilobytes lie as they are stored. The scales of 512 values follow every second step. LDS and the barriers bound it:
+// 8192 x 2048 x 7168 takes 62 to 72 us, 3.4 to 3.9 PFLOP/s of the 8.4 that the instructions reach alone, 17 of them the
+// start and the stores; without loads the same loop takes 54.
 template <int WM, int WN, int FM, int FN, bool GLU>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2))) void k_mx_tile4(MxMulArgs a) {
     constexpr int TM = WM * FM * 16, FH = GLU ? FN / 2 : FN, NS = WN * FH, NO = NS * 16, NW = WM * WN, TS = WN * FN;

