@@ -482,7 +482,10 @@ def check_choice(ids, weights, logits, k, score, bias, ngroup, keep, renorm, sca
 
 @pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("ntok,nexp,k,ngroup,keep", [(1, 8, 2, 1, 1), (5, 1, 1, 1, 1), (7, 64, 6, 1, 1), (130, 100, 8, 1, 1),
-                                                     (33, 256, 8, 8, 4), (9, 160, 6, 8, 3), (6, 384, 8, 1, 1),
+                                                     (33, 256, 8, 8, 4), (9, 160, 6, 8, 3), (6, 384, 8, 1, 1), (70, 384, 16, 1, 1),
+                                                     (9, 300, 17, 4, 3), (9, 640, 4, 32, 9),
+                                                     (2049, 8, 2, 1, 1), (2100, 256, 8, 8, 4), (2050, 100, 7, 1, 1),
+                                                     (2053, 480, 16, 16, 5), (2051, 384, 1, 4, 1), (2050, 36, 4, 12, 5),
                                                      (3, 512, 10, 4, 2), (3, 1000, 64, 1, 1), (4, 24, 4, 12, 5)])
 def test_route(gq, ex, src, ntok, nexp, k, ngroup, keep):
     torch = torch_()
@@ -509,17 +512,36 @@ def test_route_ties_and_strides(gq, ex):
     assert ids.cpu().tolist() == [list(range(12))] * 3
 
 
+@pytest.mark.parametrize("ntok", [8, 2051])
+@pytest.mark.parametrize("nexp,k", [(64, 2), (256, 8), (384, 8), (512, 16), (384, 20), (1024, 3)])
+def test_route_where_many_reach_the_bound(gq, ex, nexp, k, ntok):
+    """keys that rise along the lanes' groups, and rows of few different values: more candidates than there is room for"""
+    torch = torch_()
+    rng = np.random.default_rng(nexp)
+    rows = [np.arange(nexp), -np.arange(nexp), np.arange(nexp) % 16, (np.arange(nexp) % 64 < 8) * 1.0, np.zeros(nexp),
+            rng.integers(0, 2, nexp), np.where(np.arange(nexp) % 16 == 3, 1.0, 0.0), np.where(rng.random(nexp) < 0.5, -0.0, 0.0)]
+    rows = [rows[i % 8] for i in range(ntok)]
+    logits = torch.from_numpy(np.stack(rows).astype(np.float32)).cuda()
+    ids, w = ex.route(gq, logits, k)
+    want = np.stack([np.argsort(-r.astype(np.float64), kind="stable")[:k] for r in rows])
+    assert np.array_equal(ids.cpu().numpy(), want)
+    check_choice(ids[:9].cpu().numpy(), w[:9].cpu().numpy(), logits[:9].cpu().numpy(), k, "softmax", None, 1, 1, True, 1.0)
+
+
+@pytest.mark.parametrize("times", [1, 400])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("with_bias", [False, True], ids=["plain", "bias"])
-def test_route_with_nothing_left(gq, ex, score, with_bias):
+def test_route_with_nothing_left(gq, ex, score, with_bias, times):
     """masked experts (minus infinity, NaN) are never taken; a row of them alone gets -1 and 0; infinities count"""
     torch = torch_()
     inf, nan = float("inf"), float("nan")
     logits = torch.tensor([[-inf] * 6, [nan] * 6, [-inf, 2.0, nan, -inf, 1.0, -inf], [0.0, inf, 1.0, 2.0, -inf, nan],
                            [-3.4e38] * 6, [-200.0, -300.0, -250.0, -400.0, -500.0, -600.0]], device="cuda")
+    logits = logits.repeat(times, 1)
     bias = torch.zeros(6, device="cuda") if with_bias else None
     ids, w = ex.route(gq, logits, 3, score=score, bias=bias)
-    ids, w = ids.cpu().tolist(), w.cpu().numpy()
+    assert torch.equal(ids, ids[:6].repeat(times, 1)) and torch.equal(w, w[:6].repeat(times, 1))
+    ids, w = ids[:6].cpu().tolist(), w[:6].cpu().numpy()
     assert ids[0] == ids[1] == [-1, -1, -1] and not w[:2].any()
     assert ids[2] == [1, 4, -1] and w[2, 2] == 0 and abs(w[2].sum() - 1) < 1e-6
     assert ids[3][0] == 1 and np.isfinite(w[3]).all()

@@ -101,13 +101,32 @@ template <int WM, int WN, int FM, int FN> void launch_tile4(bool glu, dim3 grid,
 }
 
 template <int SRC> bool launch_route(const RouteArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)((a.ntok + 3) / 4));
-    if (a.nexp <= 64) hipLaunchKernelGGL((k_route<SRC, 1>), grid, dim3(256), 0, st, a);
-    else if (a.nexp <= 128) hipLaunchKernelGGL((k_route<SRC, 2>), grid, dim3(256), 0, st, a);
-    else if (a.nexp <= 256) hipLaunchKernelGGL((k_route<SRC, 4>), grid, dim3(256), 0, st, a);
-    else if (a.nexp <= 384) hipLaunchKernelGGL((k_route<SRC, 6>), grid, dim3(256), 0, st, a);
-    else if (a.nexp <= 512) hipLaunchKernelGGL((k_route<SRC, 8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_route<SRC, 16>), grid, dim3(256), 0, st, a);
+    const dim3 grid16((unsigned)((a.ntok + 15) / 16)), grid((unsigned)((a.ntok + 3) / 4));
+#define RT16(P) hipLaunchKernelGGL((k_route16<SRC, P>), grid16, dim3(256), 0, st, a)
+#define RT64(P) hipLaunchKernelGGL((k_route<SRC, P>), grid, dim3(256), 0, st, a)
+    // Kernel times with 16 and 64 lanes a token: 512 tokens of 384 experts 7.7 and 5.5 us, 4096 8.0 and 7.6, 8192 8.8 and
+    // 10.9, 16384 11.7 and 16.2; of 64 experts, 512 tokens 4.2 and 4.2, 2048 4.0 and 4.4, 4096 4.3 and 5.6, 16384 5.6 and 12.
+    if (a.ntok > 2048 && a.k <= 16 && a.ngroup <= 16 && a.nexp <= 512) {
+        if (a.nexp <= 64) RT16(4);
+        else if (a.nexp <= 128) RT16(8);
+        else if (a.nexp <= 256) RT16(16);
+        else if (a.nexp <= 384) RT16(24);
+        else RT16(32);
+    } else if (a.nexp <= 64) {
+        RT64(1);
+    } else if (a.nexp <= 128) {
+        RT64(2);
+    } else if (a.nexp <= 256) {
+        RT64(4);
+    } else if (a.nexp <= 384) {
+        RT64(6);
+    } else if (a.nexp <= 512) {
+        RT64(8);
+    } else {
+        RT64(16);
+    }
+#undef RT16
+#undef RT64
     return hipGetLastError() == hipSuccess;
 }
 
@@ -271,7 +290,8 @@ extern "C" int gpuq_route_dev(int type, const void *d_logits, int64_t ntok, int6
     if (((uintptr_t)d_logits & (type_size(type) - 1)) || ((uintptr_t)d_bias & 3) || ((uintptr_t)d_ids & 3) ||
         ((uintptr_t)d_weights & 3))
         return 1;
-    const RouteArgs a = {d_logits, ld, d_bias, d_ids, d_weights, ntok, nexp, k, ngroup, keep, scale, sigmoid != 0, renorm != 0};
+    const RouteArgs a = {d_logits, ld, d_bias, d_ids, d_weights, ntok, nexp, k, ngroup, keep, scale, sigmoid != 0, renorm != 0,
+                         mx_div((uint32_t)(nexp / ngroup))};
     const hipStream_t st = (hipStream_t)stream;
     const bool ok = type == T_F32 ? launch_route<T_F32>(a, st) : type == T_F16 ? launch_route<T_F16>(a, st)
                                                                               : launch_route<T_BF16>(a, st);

@@ -6,7 +6,7 @@
 // of the taken scores with `renorm`. A NaN logit or key counts as minus infinity, which is never taken: what is left
 // over gets id -1 and weight 0.
 #pragma once
-#include "common.cuh"
+#include "mxfp4.cuh"
 
 struct RouteArgs {
     const void *logits;
@@ -18,6 +18,7 @@ struct RouteArgs {
     int nexp, k, ngroup, keep;
     float scale;
     int sigmoid, renorm;
+    MxDiv per;                  // experts of a group
 };
 
 // the other lane of each pair at distance 1, 2, 4, 8 (within rows of 16 lanes, as a reduction needs it), 16 and 32
@@ -64,12 +65,214 @@ template <int SRC> DEV float rt_load(const void *p, int64_t i) {
 
 #define RT_NONE (-__builtin_inff())
 
-// One wave a token; lane l holds experts l, l + 64, ... The k largest keys are found in one pass: the smallest of the
-// maxima of at least k groups of lanes is reached by at least k keys, so only the keys that reach it (about three times
-// k) can be among them; they are moved to one a lane in index order and each counts the ones ahead of it. Where more than
-// 64 reach it, the largest is taken k times instead. A score is computed only where it is needed: logits order the
-// experts by themselves unless a bias or groups come in, and the sum over all cancels with renorm. Instructions bound
-// it: 16384 tokens of 384 experts take 16.5 us (taking the largest key k times over took 26.6), 0.8 TB/s.
+// The k largest keys are found in one pass: a bound that at least k keys reach (the k-th largest of the lanes' maxima)
+// leaves about half as many again, which are moved to LDS in index order and each count the ones ahead of them. Where more
+// reach it than there is room for, the largest is taken k times instead. A score is computed only where it is needed:
+// logits order the experts by themselves unless a bias or groups come in, and the sum over all cancels with renorm.
+
+// what the wave's lanes wrote to LDS is there for the others (LDS takes a wave's instructions in order; this keeps the
+// compiler to it)
+DEV void rt_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// keys as whole numbers in the same order, minus zero with zero
+DEV int rt_order(float f) {
+    const int b = (int)fbits(f + 0.f);
+    return b < 0 ? b ^ 0x7fffffff : b;
+}
+#define RT_LEAST ((int)0x80000000)
+
+// 16 lanes a token, four tokens a wave; lane l holds experts l, l + 16, ... Reductions then stay within a row of lanes
+// and an instruction serves four tokens, but a token's own way through is longer: 16384 tokens of 384 experts take 11.7 us, with
+// a wave a token (below) 16.2; one token of 256 in 8 groups 9.1 and 5.2. k and the groups at most 16, at most 512 experts.
+template <int SRC, int P>
+__global__ __launch_bounds__(256) void k_route16(RouteArgs a) {
+    constexpr int ROOM = 64;
+    __shared__ float keys[16][17 * P], gs[16][16];          // (one place in 16 left out, so that groups start in other banks)
+    __shared__ __align__(16) int ck[16][ROOM];
+    __shared__ short ci[16][ROOM];
+    const int tid = threadIdx.x, l = tid & 15, q = tid >> 4, row4 = q & 3;       // token q of the workgroup's 16
+    const int64_t t = (int64_t)blockIdx.x * 16 + q;
+    const bool live = t < a.ntok;
+    const int64_t row = (live ? t : a.ntok - 1) * a.ld;
+    // a lane's 16 bits of a wave's vote
+    auto vote = [&](bool on) {
+        const uint64_t m = __ballot(on);
+        const uint32_t w = row4 & 2 ? (uint32_t)(m >> 32) : (uint32_t)m;
+        return (w >> (16 * (row4 & 1))) & 0xffffu;
+    };
+    auto row_max = [](float v) {
+        v = fmaxf(v, rt_other<1>(v));
+        v = fmaxf(v, rt_other<2>(v));
+        v = fmaxf(v, rt_other<4>(v));
+        return fmaxf(v, rt_other<8>(v));
+    };
+    auto row_sum = [](float v) {
+        v += rt_other<1>(v);
+        v += rt_other<2>(v);
+        v += rt_other<4>(v);
+        return v + rt_other<8>(v);
+    };
+    float x[P], key[P];
+    float mx = RT_NONE;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const int e = j * 16 + l;
+        x[j] = e < a.nexp ? rt_load<SRC>(a.logits, row + e) : RT_NONE;
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        x[j] = x[j] == x[j] ? fminf(x[j], 3.402823466e38f) : RT_NONE;
+        mx = fmaxf(mx, x[j]);
+    }
+    const bool by_logit = !a.bias && a.ngroup == 1;
+    float z = 1.f;
+    if (!a.sigmoid) {
+        mx = row_max(mx);
+        if (!by_logit || !a.renorm) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < P; ++j) s += x[j] == RT_NONE ? 0.f : expf(x[j] - mx);
+            z = row_sum(s);
+            z = z > 0.f ? z : 1.f;
+        }
+    }
+    auto score = [&](float v) { return v == RT_NONE ? 0.f : a.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - mx) / z; };
+    if (by_logit) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) key[j] = x[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int e = j * 16 + l;
+            float v = score(x[j]);
+            if (a.bias && e < a.nexp) v += a.bias[e];
+            key[j] = v == v && x[j] != RT_NONE ? v : RT_NONE;
+        }
+    }
+    if (a.ngroup > 1) {         // (uniform)
+#pragma unroll
+        for (int j = 0; j < P; ++j) keys[q][j * 17 + l] = key[j];
+        rt_wave_sync();
+        float best = RT_NONE, next = RT_NONE;
+        if (l < a.ngroup) {
+#pragma unroll 8
+            for (uint32_t i = 0; i < a.per.d; ++i) {
+                const uint32_t e = l * a.per.d + i;
+                const float v = keys[q][e + e / 16];
+                next = fmaxf(next, fminf(best, v));
+                best = fmaxf(best, v);
+            }
+        }
+        const float g = next == RT_NONE ? best : best + next;
+        gs[q][l] = g;
+        rt_wave_sync();
+        int ahead = 0;          // groups that come before this one
+#pragma unroll 8
+        for (int i = 0; i < a.ngroup; ++i) ahead += gs[q][i] > g || (gs[q][i] == g && i < l);
+        const uint32_t kept = vote(l < a.ngroup && ahead < a.keep);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int e = j * 16 + l;
+            if (e < a.nexp && !((kept >> a.per.div((uint32_t)e)) & 1)) key[j] = RT_NONE;
+        }
+    }
+    float top = key[0];
+#pragma unroll
+    for (int j = 1; j < P; ++j) top = fmaxf(top, key[j]);
+    int above = 0;              // the lanes of the token whose maximum is larger
+#define RT_TURN(N) above += ffrom((uint32_t)__builtin_amdgcn_mov_dpp((int)fbits(top), 0x120 + N, 0xf, 0xf, true)) > top
+    RT_TURN(1); RT_TURN(2); RT_TURN(3); RT_TURN(4); RT_TURN(5); RT_TURN(6); RT_TURN(7); RT_TURN(8);
+    RT_TURN(9); RT_TURN(10); RT_TURN(11); RT_TURN(12); RT_TURN(13); RT_TURN(14); RT_TURN(15);
+#undef RT_TURN
+    const float bound = -row_max(above < a.k ? -top : RT_NONE);
+#pragma unroll
+    for (int i = 0; i < ROOM / 16; ++i) ck[q][ROOM / 16 * l + i] = RT_LEAST;
+    rt_wave_sync();
+    int n = 0;                  // the keys that reach it (none of minus infinity), in index order
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const bool on = key[j] >= bound && key[j] != RT_NONE;
+        const uint32_t who = vote(on);
+        const int at = n + __popc(who & ((1u << l) - 1));
+        if (on && at < ROOM) {
+            ck[q][at] = rt_order(key[j]);
+            ci[q][at] = (short)(j * 16 + l);
+        }
+        n += __popc(who);
+    }
+    rt_wave_sync();
+    int most = n;               // of the wave's four tokens
+    most = imax(most, __shfl_xor(most, 16, 64));
+    most = imax(most, __shfl_xor(most, 32, 64));
+    most = __builtin_amdgcn_readfirstlane(most);
+    int id = -1;                // of the token's l-th choice
+    if (most <= ROOM) {
+        // a candidate from before is ahead of one if it is not less, one from behind if it is more
+        int mine[ROOM / 16], ahead[ROOM / 16];
+#pragma unroll
+        for (int c = 0; c < ROOM / 16; ++c) {
+            mine[c] = ck[q][16 * c + l];
+            ahead[c] = 0;
+        }
+        auto count = [&](auto rounds) {                     // candidates in rounds of 16
+            constexpr int R = decltype(rounds)::value;
+#pragma unroll
+            for (int i = 0; i < 16 * R; i += 4) {
+                const int w[4] = {ck[q][i], ck[q][i + 1], ck[q][i + 2], ck[q][i + 3]};
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int c = 0; c < R; ++c)
+                        ahead[c] += w[u] > ((i + u) / 16 < c || ((i + u) / 16 == c && (i + u) % 16 < l) ? mine[c] - 1 : mine[c]);
+            }
+        };
+        if (most <= 16) count(IntC<1>{});
+        else if (most <= 32) count(IntC<2>{});
+        else count(IntC<4>{});              // (rare)
+        short e[ROOM / 16];
+#pragma unroll
+        for (int c = 0; c < ROOM / 16; ++c) e[c] = ci[q][16 * c + l];
+        rt_wave_sync();
+        ci[q][l] = -1;
+        rt_wave_sync();
+#pragma unroll
+        for (int c = 0; c < ROOM / 16; ++c)
+            if (mine[c] != RT_LEAST && ahead[c] < a.k) ci[q][ahead[c]] = e[c];
+        rt_wave_sync();
+        id = l < a.k ? ci[q][l] : -1;
+    } else {
+        for (int r = 0; r < a.k; ++r) {
+            float v = key[0];
+#pragma unroll
+            for (int j = 1; j < P; ++j) v = fmaxf(v, key[j]);
+            const float m = row_max(v);
+            float first = 1e9f;                             // (expert numbers are exact)
+#pragma unroll
+            for (int j = P - 1; j >= 0; --j) first = key[j] == m && m != RT_NONE ? (float)(j * 16 + l) : first;
+            first = -row_max(-first);
+            const int e = first < 1e9f ? (int)first : -1;
+#pragma unroll
+            for (int j = 0; j < P; ++j)
+                if (j * 16 + l == e) key[j] = RT_NONE;
+            if (l == r) id = e;
+        }
+    }
+    float my = 0.f;
+    if (id >= 0) my = score(fminf(rt_load<SRC>(a.logits, row + id), 3.402823466e38f));
+    const float sum = row_sum(my);
+    if (live && l < a.k) {
+        const float w = !a.renorm ? my : sum > 0.f ? my / sum : 0.f;
+        a.ids[t * a.k + l] = id;
+        a.weights[t * a.k + l] = w * a.scale;
+    }
+}
+
+// One wave a token, for few tokens or more experts, choices or groups; lane l holds experts l, l + 64, ... The bound is the
+// smallest of the maxima of k or more groups of lanes.
 template <int SRC, int P>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     __shared__ float keys[4][64 * P], gs[4][64];
@@ -117,26 +320,25 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     if (a.ngroup > 1) {         // (uniform)
 #pragma unroll
         for (int j = 0; j < P; ++j) keys[wave][j * 64 + lane] = key[j];
-        __builtin_amdgcn_wave_barrier();
-        const int per = a.nexp / a.ngroup;
+        rt_wave_sync();
         float best = RT_NONE, next = RT_NONE;
         if (lane < a.ngroup) {
-            for (int i = 0; i < per; ++i) {
-                const float v = keys[wave][lane * per + i];
+            for (uint32_t i = 0; i < a.per.d; ++i) {
+                const float v = keys[wave][lane * a.per.d + i];
                 next = fmaxf(next, fminf(best, v));
                 best = fmaxf(best, v);
             }
         }
         const float g = next == RT_NONE ? best : best + next;
         gs[wave][lane] = g;
-        __builtin_amdgcn_wave_barrier();
+        rt_wave_sync();
         int ahead = 0;          // groups that come before this one
         for (int i = 0; i < a.ngroup; ++i) ahead += gs[wave][i] > g || (gs[wave][i] == g && i < lane);
         const uint64_t kept = __ballot(lane < a.ngroup && ahead < a.keep);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const int e = j * 64 + lane;
-            if (e < a.nexp && !((kept >> (e / per)) & 1)) key[j] = RT_NONE;
+            if (e < a.nexp && !((kept >> a.per.div((uint32_t)e)) & 1)) key[j] = RT_NONE;
         }
     }
     float top = key[0];
@@ -149,17 +351,15 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
         const bool on = key[j] >= bound && key[j] != RT_NONE;
         const uint64_t who = __ballot(on);
         const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-        if (on && at < 64) cand[wave][at] = make_int2((int)fbits(key[j]), j * 64 + lane);
+        if (on && at < 64) cand[wave][at] = make_int2(rt_order(key[j]), j * 64 + lane);
         n += __popcll(who);
     }
-    __builtin_amdgcn_wave_barrier();
+    rt_wave_sync();
     int rank = 64, id = -1;     // this lane's candidate, if it is among the k
     if (n <= 64) {
-        // keys as whole numbers in the same order: one from before this lane is ahead if it is not less, one from behind if
-        // it is more (lanes past n hold less than all)
+        // one from before this lane is ahead if it is not less, one from behind if it is more
         const int2 c = cand[wave][lane];
-        const int b = c.x == (int)0x80000000 ? 0 : c.x;     // (minus zero ties with zero)
-        const int mine = lane < n ? (b < 0 ? b ^ 0x7fffffff : b) : (int)0x80000000;
+        const int mine = lane < n ? c.x : RT_LEAST;
         id = lane < n ? c.y : -1;
         int ahead = 0;
         for (int i0 = 0; i0 < n; i0 += 8) {
@@ -188,11 +388,11 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
             }
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    rt_wave_sync();
     if (lane < a.k) cid[wave][lane] = -1;
-    __builtin_amdgcn_wave_barrier();
+    rt_wave_sync();
     if (rank < a.k) cid[wave][rank] = id;
-    __builtin_amdgcn_wave_barrier();
+    rt_wave_sync();
     const int my_id = lane < a.k ? cid[wave][lane] : -1;
     float my = 0.f;
     if (my_id >= 0) {
@@ -250,7 +450,7 @@ __global__ __launch_bounds__(1024) void k_group_count(const int32_t *__restrict_
 // offsets [nexp + 1], rows [n] (the token of each sorted assignment), slots [n] (its flat index); the places past
 // offsets[nexp] (ids that name no expert) get -1. counts is null where there is one chunk. Each of the NW waves places its
 // share of the chunk, 64 assignments at a time: the place of each is the expert's next and the number of its own before it.
-// 131072 assignments of 384 experts take 3.1 us to count and 10.6 to place, most of it the counts of all chunks on their way.
+// 131072 assignments of 384 experts take 3.1 us to count and 10.6 to place, latency: loads, counts, scan and eight rounds.
 template <int NW>
 __global__ __launch_bounds__(NW * 64) void k_group_place(const int32_t *__restrict__ ids, int64_t n, int k, int nexp,
                                                          int64_t chunk, const int32_t *__restrict__ counts,
