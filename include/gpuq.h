@@ -176,8 +176,8 @@ size_t gpuq_mxfp4_matmul_work(int x_type, int glu, int64_t nx, int64_t nmat, int
                               int64_t m);
 
 /* Products of rows with MXFP4 matrices d_w [nmat][ne1][ne0] (tiles): y[r] = x[d_rows[r]] w[e]^T for the rows
- * d_offsets[e] <= r < d_offsets[e + 1] of matrix e (int32, device; nmat 1: d_offsets may be NULL, all m rows). d_rows NULL:
- * x[r]. With d_up (tiles, the same sizes) SwiGLU: y = g / (1 + exp(-g)) * u, g of d_w and u of d_up. x_type: BF16, F16,
+ * d_offsets[e] <= r < d_offsets[e + 1] of matrix e (int32, device, ascending from 0: rows that two matrices or none of
+ * them claim otherwise are not defined; nmat 1: d_offsets may be NULL, all m rows). d_rows NULL: x[r]. With d_up (tiles, the same sizes) SwiGLU: y = g / (1 + exp(-g)) * u, g of d_w and u of d_up. x_type: BF16, F16,
  * F32 [nx][ld] (rows 16-byte aligned; no bit of x or w is rounded away, sums in f32) or MXFP4 rows (39, ld = ne0).
  * y_type F32, F16 or BF16: d_y [m][ne1]. A row that no matrix has (r >= d_offsets[nmat]) or whose d_rows names no row of x
  * is zero. A scale of 255 is NaN (ggml's to_float takes it for 2^128). At most 65534 matrices and 2^30

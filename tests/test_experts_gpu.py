@@ -663,3 +663,18 @@ def test_refusals(gq, ex):
         with pytest.raises(ValueError):
             call()
     torch.cuda.synchronize()
+
+
+def test_a_matrix_of_other_bytes_is_refused(gq, ex):
+    torch = torch_()
+    x = torch.zeros(4, 512, dtype=torch.bfloat16, device="cuda")
+    data = torch.zeros(32 * 512 // 32 * 17, dtype=torch.uint8, device="cuda")
+    good, rows = ex.Packed(data, 1, 32, 512), ex.quantize(gq, x)
+    assert not ex.matmul(gq, x, good).any() and not ex.matmul(gq, rows, good, up=good).any()
+    short = good._replace(data=data[:-16])
+    for call in (lambda: ex.matmul(gq, x, short), lambda: ex.matmul(gq, x, good, up=short),
+                 lambda: ex.matmul(gq, x, good._replace(nmat=2), group=ex.Group(torch.zeros(3, dtype=torch.int32, device="cuda"),
+                                                                                torch.zeros(4, dtype=torch.int32, device="cuda"), None)),
+                 lambda: ex.matmul(gq, rows._replace(n=5), good)):
+        with pytest.raises(ValueError):
+            call()

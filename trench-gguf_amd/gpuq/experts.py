@@ -129,6 +129,10 @@ def matmul(gq, x, w, group=None, up=None, out_dtype=torch.float32):
         dev = x.device
     if ncol != w.ne0 or (up is not None and up[1:] != w[1:]) or out_dtype not in TYPES:
         raise ValueError("sizes or types of x, w and up do not fit")
+    size = _bytes(gq, TILES, *w[1:])
+    if w.data.numel() != size or (up is not None and up.data.numel() != size) or \
+            (typ == MXFP4 and x.data.numel() != _bytes(gq, ROWS, 1, n, ncol)):
+        raise ValueError("w, up or x do not hold the bytes of their sizes")
     offsets = rows = None
     m = n
     if group is not None:
