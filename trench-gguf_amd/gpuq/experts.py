@@ -53,12 +53,13 @@ def _group_work(gq, *sizes):
 
 def _rows(x):
     """(type, pointer, rows, columns, elements from row to row) of a 2-d float tensor whose rows are contiguous"""
-    if x.dim() != 2 or x.dtype not in TYPES or not x.is_cuda:
+    typ = TYPES.get(x.dtype)
+    if typ is None or x.dim() != 2 or not x.is_cuda:
         raise ValueError("expected a 2-d F32 / F16 / BF16 tensor on the GPU")
-    if x.stride(1) != 1 and x.shape[1] > 1:
+    (n, ncol), (ld, step) = x.shape, x.stride()
+    if step != 1 and ncol > 1:
         raise ValueError("rows must be contiguous")
-    ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    return TYPES[x.dtype], x.data_ptr(), x.shape[0], x.shape[1], ld
+    return typ, x.data_ptr(), n, ncol, ld if n > 1 else ncol
 
 
 def pack(gq, blocks, nmat, ne1, ne0):
@@ -122,32 +123,32 @@ def matmul(gq, x, w, group=None, up=None, out_dtype=torch.float32):
 
     Without a group m = n and w is one matrix; with one (Group, from `group`) output row r is x[group.rows[r]] times the
     matrix whose offsets hold r, zero where none does. up: a second Packed like w, for silu(x w^T) * (x up^T)."""
+    data, nmat, ne1, ne0 = w
     if isinstance(x, Rows):
-        typ, ptr, n, ncol, ld, dev = MXFP4, x.data.data_ptr(), x.n, x.ncol, x.ncol, x.data.device
+        (x, n, ncol), typ = x, MXFP4
+        ptr, ld = x.data_ptr(), ncol
     else:
         typ, ptr, n, ncol, ld = _rows(x)
-        dev = x.device
-    if ncol != w.ne0 or (up is not None and up[1:] != w[1:]) or out_dtype not in TYPES:
+    y_type, dev = TYPES.get(out_dtype), x.device
+    if ncol != ne0 or (up is not None and up[1:] != w[1:]) or y_type is None:
         raise ValueError("sizes or types of x, w and up do not fit")
-    size = _bytes(gq, TILES, *w[1:])
-    if w.data.numel() != size or (up is not None and up.data.numel() != size) or \
-            (typ == MXFP4 and x.data.numel() != _bytes(gq, ROWS, 1, n, ncol)):
+    size = _bytes(gq, TILES, nmat, ne1, ne0)
+    if data.numel() != size or (up is not None and up.data.numel() != size) or \
+            (typ == MXFP4 and x.numel() != _bytes(gq, ROWS, 1, n, ncol)):
         raise ValueError("w, up or x do not hold the bytes of their sizes")
     offsets = rows = None
     m = n
     if group is not None:
         offsets, rows, m = _index(group.offsets, "offsets"), _index(group.rows, "rows"), group.rows.numel()
-        if group.offsets.numel() != w.nmat + 1:
+        if group.offsets.numel() != nmat + 1:
             raise ValueError("offsets must be one longer than the stack")
-    y = torch.empty((m, w.ne1), dtype=out_dtype, device=dev)
-    size = _work(gq, typ, int(up is not None), n, w.nmat, w.ne1, w.ne0, int(group is not None), m)
+    y = torch.empty((m, ne1), dtype=out_dtype, device=dev)
+    size = _work(gq, typ, up is not None, n, nmat, ne1, ne0, group is not None, m)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    got = gq.gpuq_mxfp4_matmul_dev(typ, ptr, n, ld, w.data.data_ptr(), None if up is None else up.data.data_ptr(),
-                                   w.nmat, w.ne1, w.ne0, offsets, rows, m, TYPES[out_dtype], y.data_ptr(),
-                                   work.data_ptr() if size else None, _raw_stream(dev.index))
-    if not got:
-        raise ValueError("gpuq_mxfp4_matmul_dev refused %d x %d rows and %d x %d x %d weights" %
-                         (n, ncol, w.nmat, w.ne1, w.ne0))
+    if not gq.gpuq_mxfp4_matmul_dev(typ, ptr, n, ld, data.data_ptr(), None if up is None else up.data.data_ptr(), nmat,
+                                    ne1, ne0, offsets, rows, m, y_type, y.data_ptr(), work.data_ptr() if size else None,
+                                    _raw_stream(dev.index)):
+        raise ValueError("gpuq_mxfp4_matmul_dev refused %d x %d rows and %d x %d x %d weights" % (n, ncol, nmat, ne1, ne0))
     return y
 
 
