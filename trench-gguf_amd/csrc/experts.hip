@@ -61,7 +61,7 @@ template <int NF> void launch_rows(int x_type, bool glu, const MxMulArgs &a, hip
 // tile kernels read them once for 64 to 256, and where their tiles are fewer than the GPU takes at once, they split k and
 // join the partial sums. Both sides of each bound (us; experts of 2048 x 7168, 64 of them, 8 a token):
 //   8 rows a group on average, at most: k_mx_rows 112, tiles of 64 rows 120; at 16 166 and 124, at 1 67 and 104.
-//   One matrix: 16 rows 10.8 in k_mx_rows, 17 rows 16.8 in split tiles (unsplit 73).
+//   One matrix: 16 rows 10.8 in k_mx_rows, 17 rows 13.1 in split tiles, 4.6 of it the join (unsplit 73).
 //   Tiles of 128 rows from 1024 of them on, two rounds of two a CU: 4096 rows of 2048 x 7168 (256 tiles) 116, with 64 rows
 //   98; 64 experts of 512 rows, SwiGLU (4600) 1.61 ms, with 64 rows 1.64.
 //   MXFP4 rows: 256 x 256 tiles where each group has 256 rows and they fill the GPU (8192 rows 72, with 128 x 128 78).
@@ -275,7 +275,7 @@ extern "C" size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx,
         else if (plan.kind == 3) launch_tile4<2, 4, 4, 2>(glu, grid, a, st);
         else launch_tile4<2, 4, 8, 4>(glu, grid, a, st);
         if (a.part)
-            hipLaunchKernelGGL(k_mx_join, dim3((unsigned)((m * ((ne1 + 3) / 4) + 255) / 256)), dim3(256), 0, st, a, plan.split);
+            hipLaunchKernelGGL(k_mx_join, dim3((unsigned)((m * ((ne1 + 3) / 4) + 63) / 64)), dim3(64), 0, st, a, plan.split);
     }
     return hipGetLastError() == hipSuccess ? (size_t)(m * ne1 * type_size(y_type)) : 0;
 }

@@ -118,13 +118,14 @@ DEV void mx_part4(const MxMulArgs &a, int h, int64_t row, int64_t n, const float
 }
 
 // the sum of the partial sums, in order; a thread 4 outputs of a row, a row's pieces beyond its end left out
-__global__ __launch_bounds__(256) void k_mx_join(MxMulArgs a, int split) {
-    const int64_t per = (a.ne1 + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(64) void k_mx_join(MxMulArgs a, int split) {
+    const int64_t per = (a.ne1 + 3) / 4, i = (int64_t)blockIdx.x * 64 + threadIdx.x;
     if (i >= a.m * per) return;
     const int64_t row = i / per, n = i % per * 4, plane = a.m * a.ne1;
     const int mats = a.u ? 2 : 1;
     float v[2][4] = {};
-    for (int z = 0; z < split; ++z) {
+#pragma unroll 8
+    for (int z = 0; z < split; ++z) {            // (many loads in flight)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (h >= mats) continue;
@@ -402,7 +403,7 @@ DEV void mx_sync() {
 // by value. lds: the loop's buffers, free by now.
 template <int SIZE, int WM, int WN, int FM, int FN, bool GLU>
 DEV void mx_store_tile(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0, int64_t r1, int64_t s0, uint8_t *lds) {
-    constexpr int FH = GLU ? FN / 2 : FN, NO = WN * FH * 16, GC = FM / 4, CR = WM * GC * 16;
+    constexpr int FH = GLU ? FN / 2 : FN, NO = WN * FH * 16, GC = FM < 4 ? 1 : FM / 4, CR = WM * GC * 16;
     constexpr int RB = NO * SIZE + 16, PER = 16 / SIZE, PIECES = NO / PER;      // a row in LDS; values and pieces of a row
     const int tid = threadIdx.x, lane = lane_id(), q = lane >> 4, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
     const bool whole = a.ne1 % PER == 0;
@@ -530,14 +531,14 @@ DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int
         uint8_t *buf = xs + (s & 1) * (TM * 256);
         if ((int64_t)s * 128 + 128 > a.kx) {                // (the last step, of rows that end inside it)
 #pragma unroll
-            for (int i = j * LD / 4; i < (j + 1) * LD / 4; ++i) {
+            for (int i = (j * LD + 3) / 4; i < ((j + 1) * LD + 3) / 4; ++i) {
                 const int p = (lane & 15) ^ (((wave * LD + i) * 4 + (lane >> 4)) & 15);
                 const bool in = (int64_t)s * 128 + 8 * (4 * (p & 3) + (p >> 2)) < a.kx;
                 mx_to_lds(in ? xp[i] : (const uint8_t *)mx_zero, buf + (wave * LD + i) * 1024);
             }
         } else {
 #pragma unroll
-            for (int i = j * LD / 4; i < (j + 1) * LD / 4; ++i) {
+            for (int i = (j * LD + 3) / 4; i < ((j + 1) * LD + 3) / 4; ++i) {
                 mx_to_lds(xp[i], buf + (wave * LD + i) * 1024);
                 xp[i] += 256;
             }
@@ -594,7 +595,8 @@ DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int
     mx_epilogue<1, WN, FM, FN, GLU>(a, acc, r0, r1, s0, xs);
 }
 
-// Tiles of FM x 16 rows; one with no more than half of them takes half the fragments
+// Tiles of FM x 16 rows; one with no more than half of them takes half the fragments (64 experts of some 20 rows of 2048 x 7168
+// 153 -> 135 us, 17 rows of one 10.5 -> 8.5)
 template <int WN, int FM, int FN, bool GLU>
 __global__ __launch_bounds__(WN * 64) __attribute__((amdgpu_waves_per_eu(2))) void k_mx_tile(MxMulArgs a) {
     constexpr int NS = WN * FN / (GLU ? 2 : 1);
@@ -604,7 +606,7 @@ __global__ __launch_bounds__(WN * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     if (!mx_tile<FM * 16>(a, (int)((a.strips + NS - 1) / NS), e, r0, r1, col)) return;
     const int64_t s0 = (int64_t)col * NS;                   // the tile's first strip
     if (e == a.nmat) mx_clear<NS * 16>(a, r0, r1, s0 * 16, WN * 64);
-    else if (FM == 8 && r1 - r0 <= FM * 8) mx_tile_body<WN, FM == 8 ? FM / 2 : FM, FN, GLU>(a, e, r0, r1, s0, xs);
+    else if (r1 - r0 <= FM * 8) mx_tile_body<WN, FM / 2, FN, GLU>(a, e, r0, r1, s0, xs);
     else mx_tile_body<WN, FM, FN, GLU>(a, e, r0, r1, s0, xs);
 }
 
