@@ -21,6 +21,7 @@
 
 typedef __bf16 mx_bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 mx_bf2 __attribute__((ext_vector_type(2)));
+typedef int mx_i4 __attribute__((ext_vector_type(4)));
 typedef float mx_f4 __attribute__((ext_vector_type(4)));
 
 #define MX_PAD 512
@@ -50,6 +51,12 @@ DEV uint32_t mx_spread(uint32_t h) {
 DEV uint32_t mx_gather(uint32_t b) {
     b = (b | (b >> 4)) & 0x00ff00ffu;
     return (b | (b >> 8)) & 0xffffu;
+}
+
+// 16 bytes to where nothing reads them soon: written through, or they would push what is being read out of L2 and leave all
+// at once at a kernel's end
+DEV void mx_stream(void *p, uint4 v) {
+    __builtin_nontemporal_store(mx_i4{(int)v.x, (int)v.y, (int)v.z, (int)v.w}, (mx_i4 *)p);
 }
 
 // 8 source values as they are stored

@@ -440,7 +440,7 @@ DEV void mx_store_tile(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r
             const int lr = i / PIECES, p = i % PIECES, w = lr / (GC * 16);
             const int64_t r = r0 + (w * FM + g0) * 16 + lr % (GC * 16), n = s0 * 16 + p * PER;
             if (r < r1 && n < a.ne1)
-                *(uint4 *)((uint8_t *)a.y + (r * a.ne1 + n) * SIZE) = *(const uint4 *)(lds + lr * RB + p * 16);
+                mx_stream((uint8_t *)a.y + (r * a.ne1 + n) * SIZE, *(const uint4 *)(lds + lr * RB + p * 16));
         }
         __syncthreads();
     }
