@@ -678,3 +678,18 @@ def test_a_matrix_of_other_bytes_is_refused(gq, ex):
                  lambda: ex.matmul(gq, rows._replace(n=5), good)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
+def test_many_rows_round_as_few_do(gq, ex, src):
+    """more rows than the caches hold take loads and stores of their own kind"""
+    torch = torch_()
+    n, ncol = (129 << 20) // (512 * (4 if src == "f32" else 2)) + 3, 512
+    torch.manual_seed(7)
+    x = torch.randn(n, ncol, device="cuda").to({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[src])
+    x[n // 3] = float("inf")
+    x[n // 3 + 1, ::7] = float("nan")
+    blocks, values = ex.quantize_blocks(gq, x, values=True)
+    for a in range(0, n, n // 3):
+        b, v = ex.quantize_blocks(gq, x[a:a + n // 3], values=True)
+        assert torch.equal(blocks[a:a + n // 3], b) and torch.equal(values[a:a + n // 3], v)

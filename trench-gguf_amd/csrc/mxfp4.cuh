@@ -21,7 +21,7 @@
 
 typedef __bf16 mx_bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 mx_bf2 __attribute__((ext_vector_type(2)));
-typedef int mx_i4 __attribute__((ext_vector_type(4)));
+typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
 typedef float mx_f4 __attribute__((ext_vector_type(4)));
 
 #define MX_PAD 512
@@ -56,16 +56,17 @@ DEV uint32_t mx_gather(uint32_t b) {
 // 16 bytes to where nothing reads them soon: written through, or they would push what is being read out of L2 and leave all
 // at once at a kernel's end
 DEV void mx_stream(void *p, uint4 v) {
-    __builtin_nontemporal_store(mx_i4{(int)v.x, (int)v.y, (int)v.z, (int)v.w}, (mx_i4 *)p);
+    __builtin_nontemporal_store(mx_u4{v.x, v.y, v.z, v.w}, (mx_u4 *)p);
 }
 
-// 8 source values as they are stored
+// 8 source values as they are stored; STREAM: they are read once and not kept
 template <int SRC> struct MxRaw { uint32_t w[SRC == T_F32 ? 8 : 4]; };
-template <int SRC> DEV MxRaw<SRC> mx_load8(const void *src, int64_t i) {
+template <int SRC, bool STREAM = false> DEV MxRaw<SRC> mx_load8(const void *src, int64_t i) {
     MxRaw<SRC> r;
 #pragma unroll
     for (int k = 0; k < (SRC == T_F32 ? 2 : 1); ++k) {
-        const uint4 a = *((const uint4 *)((const uint8_t *)src + i * (SRC == T_F32 ? 4 : 2)) + k);
+        const mx_u4 *at = (const mx_u4 *)((const uint8_t *)src + i * (SRC == T_F32 ? 4 : 2)) + k;
+        const mx_u4 a = STREAM ? __builtin_nontemporal_load(at) : *at;
         r.w[4 * k] = a.x;
         r.w[4 * k + 1] = a.y;
         r.w[4 * k + 2] = a.z;
@@ -164,14 +165,15 @@ enum { MX_BLOCKS = 0, MX_ROWS = 1, MX_TILES = 2 };
 
 // quarter a of a block as the source has it, zero where it holds none: 8 values, or of MXFP4 8 bytes of codes and the scale
 template <int SRC> struct MxQuarter { MxRaw<SRC == T_MXFP4 ? T_BF16 : SRC> r; };
-template <int SRC> DEV MxQuarter<SRC> mx_source(const MxQuantArgs &p, int64_t row, uint32_t col, bool real, int a) {
+template <int SRC, bool STREAM = false>
+DEV MxQuarter<SRC> mx_source(const MxQuantArgs &p, int64_t row, uint32_t col, bool real, int a) {
     MxQuarter<SRC> v;
     if constexpr (SRC == T_MXFP4) {
         const uint8_t *blk = (const uint8_t *)p.src + (real ? row * p.nb + col : 0) * 17;
         v.r.w[2] = blk[0];
         __builtin_memcpy(&v.r.w[0], blk + 1 + 8 * (a & 1), 8);
     } else {
-        v.r = mx_load8<SRC>(p.src, (real ? row * p.ld + (int64_t)col * 32 : 0) + 8 * a);
+        v.r = mx_load8<SRC, STREAM>(p.src, (real ? row * p.ld + (int64_t)col * 32 : 0) + 8 * a);
     }
 #pragma unroll
     for (int j = 0; j < (SRC == T_F32 ? 8 : SRC == T_MXFP4 ? 3 : 4); ++j) v.r.w[j] = real ? v.r.w[j] : 0;
@@ -204,11 +206,16 @@ template <int SRC> DEV uint32_t mx_encode(int a, const MxQuarter<SRC> &q, uint32
     }
 }
 
-// blocks: four lanes a block, 8 values a lane, MX_U blocks a lane; the 17-byte blocks of a workgroup leave through LDS
+// blocks: four lanes a block, 8 values a lane, MX_U blocks a lane; the 17-byte blocks of a workgroup leave through LDS.
+// STREAM: neither the values nor what is made of them stay in the caches
 #define MX_U 4
-template <int SRC>
+template <int SRC, bool STREAM>
 __global__ __launch_bounds__(256) void k_mx_blocks(MxQuantArgs p) {
     __shared__ __align__(16) uint8_t out[MX_U * 64 * 17];
+    auto put = [](void *to, uint4 v) {
+        if (STREAM) mx_stream(to, v);
+        else *(uint4 *)to = v;
+    };
     const int tid = threadIdx.x, a = tid & 3;
     const uint32_t b0 = blockIdx.x * (MX_U * 64) + (tid >> 2);
     MxQuarter<SRC> v[MX_U];
@@ -218,14 +225,14 @@ __global__ __launch_bounds__(256) void k_mx_blocks(MxQuantArgs p) {
         const uint32_t b = b0 + 64 * u < p.nblk ? b0 + 64 * u : p.nblk - 1;
         row[u] = p.row.div(b);
         col[u] = b - row[u] * p.row.d;
-        v[u] = mx_source<SRC>(p, row[u], col[u], true, a);
+        v[u] = mx_source<SRC, STREAM>(p, row[u], col[u], true, a);
     }
 #pragma unroll
     for (int u = 0; u < MX_U; ++u) {
         uint32_t e;
         const uint32_t codes = mx_encode<SRC>(a, v[u], e);
         if (p.values && b0 + 64 * u < p.nblk)
-            *(uint4 *)(p.values + (int64_t)row[u] * p.ncol + col[u] * 32 + 8 * a) = mx_values(codes, e);
+            put(p.values + (int64_t)row[u] * p.ncol + col[u] * 32 + 8 * a, mx_values(codes, e));
         // ggml's block: e, then byte j = value j | value j + 16 << 4; lane a gets bytes 4a .. 4a + 3
         const uint32_t lo = mx_quad<0x50>(codes) >> (16 * (a & 1)), hi = mx_quad<0xFA>(codes) >> (16 * (a & 1));
         const uint32_t w = mx_spread(lo & 0xffffu) | (mx_spread(hi & 0xffffu) << 4);
@@ -240,7 +247,7 @@ __global__ __launch_bounds__(256) void k_mx_blocks(MxQuantArgs p) {
     uint8_t *d = p.dst + (int64_t)first * 17;
     for (uint32_t i = tid * 16; i < n; i += 256 * 16) {
         if (i + 16 <= n) {
-            *(uint4 *)(d + i) = *(const uint4 *)(out + i);
+            put(d + i, *(const uint4 *)(out + i));
         } else {
             for (uint32_t j = i; j < n; ++j) d[j] = out[j];
         }
