@@ -478,7 +478,7 @@ DEV void mx_epilogue(const MxMulArgs &a, const mx_f4 (&acc)[FN][FM], int64_t r0,
 // over the banks. A wave's weights go straight to its registers, a kilobyte of a strip at a time and one ahead: as codes
 // they are a quarter of what the rows take, and no two waves read the same. The matrix instructions and the power they
 // draw bound it: 64 experts of 512 rows with SwiGLU keep them busy for two thirds of the time at 1.9 GHz, 1.2 PFLOP/s of
-// the 1.4 that the library's product of BF16 rows and weights of that size reaches; 4096 x 2048 x 7168 takes 98 to 105 us,
+// the 1.4 that the library's product of BF16 rows and weights of that size reaches; 4096 x 2048 x 7168 takes 94 to 98 us,
 // the library's 107. Two workgroups a CU cover each other's waits; eight waves of one that take turns between LDS and
 // the products took 130 to 200 us there.
 template <int WN, int FM, int FN, bool GLU>
@@ -569,6 +569,9 @@ DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int
                 xv[t & 1][i] = *(const uint4 *)(b + (t % HP * 2 + i) * 4096 + (((4 * (t / HP) + q) ^ (lane & 15)) * 16));
         };
         mx_bf8 wv[FN];
+        // products come before the starts of steps of a CU's other workgroups (4096 x 2048 x 7168 99 -> 96.5 us; the larger
+        // tiles, two waves a SIMD, the same)
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int t = 0; t < 4 * HP; ++t) {
             const int j = t / HP, p = t % HP;
@@ -590,6 +593,7 @@ DEV void mx_tile_body(const MxMulArgs &a, int64_t e, int64_t r0, int64_t r1, int
             __builtin_amdgcn_sched_barrier(0);
         }
         c = next;
+        __builtin_amdgcn_s_setprio(0);
         mx_sync();
     }
     mx_epilogue<1, WN, FM, FN, GLU>(a, acc, r0, r1, s0, xs);
@@ -614,8 +618,8 @@ __global__ __launch_bounds__(WN * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
 // take a quarter of the BF16 ones' time, so both go through LDS (nothing is read twice), 256 values of k a step in two
 // buffers, and every load has a step's time. A row of x is 8 pieces of 16 bytes, piece p at p ^ (row / 2 & 7); a strip's
 // kilobytes lie as they are stored. The scales of 512 values follow every second step. LDS and the barriers bound it:
-// 8192 x 2048 x 7168 takes 62 to 72 us, 3.4 to 3.9 PFLOP/s of the 8.4 that the instructions reach alone, 17 of them the
-// start and the stores; without loads the same loop takes 54.
+// 8192 x 2048 x 7168 takes 60 to 67 us, 3.6 to 4.0 PFLOP/s of the 8.4 that the instructions reach alone, some 14 of them
+// the start and the stores (through the caches 17).
 template <int WM, int WN, int FM, int FN, bool GLU>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2))) void k_mx_tile4(MxMulArgs a) {
     constexpr int TM = WM * FM * 16, FH = GLU ? FN / 2 : FN, NS = WN * FH, NO = NS * 16, NW = WM * WN, TS = WN * FN;
