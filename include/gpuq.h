@@ -189,7 +189,7 @@ size_t gpuq_mxfp4_matmul_dev(int x_type, const void *d_x, int64_t nx, int64_t ld
 /* A router's choice: the k best of nexp experts for each token of d_logits (F32 / F16 / BF16 [ntok][nexp], ld elements
  * from row to row) -> d_ids [ntok][k] int32, best first, and d_weights [ntok][k] f32. score = softmax over all experts, or
  * sigmoid; key = score + d_bias[e] (f32; NULL: none), or the logit itself with no bias and one group. ngroup groups of
- * nexp / ngroup neighbours: a group counts by the sum of its two largest keys (or by the one it
+ * nexp / ngroup neighbours: a group counts by the sum of its two largest keys (or by the one that it
  * has) and the `keep` best groups stay. A tie goes
  * to the lowest index. weight = scale * score, over the sum of the chosen scores with renorm (zero where that is zero).
  * A NaN or minus infinity is never chosen; what is left over gets id -1 and weight 0. nexp <= 1024, k <= 64, ngroup <= 64.
